@@ -129,6 +129,45 @@ class ForgeOptimArgs(ctypes.Structure):
     ]
 
 
+class ForgeLogprobsArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("targets", ctypes.c_void_p), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64),
+                ("ld", ctypes.c_int64), ("vocab_start", ctypes.c_int64), ("vocab_total", ctypes.c_int64),
+                ("ignore_index", ctypes.c_int64), ("temperature", ctypes.c_double), ("dtype", ctypes.c_int32),
+                ("top_k", ctypes.c_int32), ("logprobs", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("top_logprobs", ctypes.c_void_p), ("top_ids", ctypes.c_void_p), ("stats", ctypes.c_void_p),
+                ("keys", ctypes.c_void_p)]
+
+
+class ForgeMultiItem(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("numel", ctypes.c_int64),
+                ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32)]
+
+
+class ForgeMultiArgs(ctypes.Structure):
+    _fields_ = [("items", ctypes.POINTER(ForgeMultiItem)), ("count", ctypes.c_int32), ("state_mode", ctypes.c_int32),
+                ("hyper", ForgeHyper), ("hyper_device", ctypes.c_void_p), ("grad_coef", ctypes.c_void_p)]
+
+
+class ForgeNormItem(ctypes.Structure):
+    _fields_ = [("grad", ctypes.c_void_p), ("numel", ctypes.c_int64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class ForgeFp8QuantizeArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("ld_x", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("block_rows", ctypes.c_int32), ("codes", ctypes.c_void_p),
+                ("ld_codes", ctypes.c_int64), ("scales", ctypes.c_void_p), ("codes_t", ctypes.c_void_p),
+                ("ld_codes_t", ctypes.c_int64), ("scales_t", ctypes.c_void_p)]
+
+
+class ForgeFp8ProductArgs(ctypes.Structure):
+    _fields_ = [("x_codes", ctypes.c_void_p), ("x_scales", ctypes.c_void_p), ("w_codes", ctypes.c_void_p),
+                ("w_scales", ctypes.c_void_p), ("y", ctypes.c_void_p), ("M", ctypes.c_int64), ("N", ctypes.c_int64),
+                ("K", ctypes.c_int64), ("ld_x", ctypes.c_int64), ("ld_w", ctypes.c_int64), ("ld_y", ctypes.c_int64),
+                ("x_scale_row", ctypes.c_int64), ("x_scale_col", ctypes.c_int64), ("w_scale_row", ctypes.c_int64),
+                ("w_scale_col", ctypes.c_int64), ("status", ctypes.c_void_p)]
+
+
 # every symbol include/forge_b200.h declares, with its ctypes signature
 _SIGNATURES = {
     "forge_wgrad_update": (ctypes.c_int, [ctypes.POINTER(ForgeWgradArgs), ctypes.c_void_p]),
@@ -157,6 +196,17 @@ _SIGNATURES = {
     "forge_rmsnorm_backward": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int32] * 2 + [ctypes.c_int64] * 5
                                + [ctypes.c_double, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "forge_rmsnorm_backward_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
+    "forge_logprobs_forward": (ctypes.c_int, [ctypes.POINTER(ForgeLogprobsArgs), ctypes.c_void_p]),
+    "forge_logprobs_join": (ctypes.c_int, [ctypes.POINTER(ForgeLogprobsArgs), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
+                                           ctypes.c_void_p]),
+    "forge_logprobs_backward": (ctypes.c_int, [ctypes.POINTER(ForgeLogprobsArgs), ctypes.c_void_p, ctypes.c_void_p,
+                                               ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "forge_multi_adamw": (ctypes.c_int, [ctypes.POINTER(ForgeMultiArgs), ctypes.c_void_p]),
+    "forge_multi_norm_scratch_bytes": (ctypes.c_size_t, [ctypes.POINTER(ForgeNormItem), ctypes.c_int32]),
+    "forge_multi_norm": (ctypes.c_int, [ctypes.POINTER(ForgeNormItem), ctypes.c_int32, ctypes.c_double, ctypes.c_void_p,
+                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "forge_fp8_quantize": (ctypes.c_int, [ctypes.POINTER(ForgeFp8QuantizeArgs), ctypes.c_void_p]),
+    "forge_fp8_product": (ctypes.c_int, [ctypes.POINTER(ForgeFp8ProductArgs), ctypes.c_void_p]),
     "forge_state_bytes": (
         ctypes.c_int,
         [ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,

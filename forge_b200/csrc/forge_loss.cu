@@ -1,0 +1,649 @@
+// Log probability of one given token per row of logits, the row's entropy and its most likely
+// alternatives, and the gradient of the first two with respect to the logits.  With z = x / temperature
+// and m any number near the row's maximum:
+//   S = sum e^(z - m)      T = sum (z - m) e^(z - m)      lse = m + log S
+//   logprob = z_t - lse    entropy = log S - T / S        p_j = e^(z_j - lse)
+//   dx_j = ( g_l (1[j = t] - p_j) - g_h p_j (log p_j + entropy) ) / temperature
+//
+// Forward: ONE pass over the logits.  Every thread keeps a running (m, S, T) of its own; m moves only
+// when a value exceeds it by more than LAZY_LOG, so rescaling is rare (S then stays below V e^LAZY_LOG
+// in fp32).  The partial results of threads, warps and CTAs are joined by the same rule.  A row belongs
+// to a CLUSTER of CTAs (1 for many rows, up to 16 for a few): the join over a long row goes through
+// distributed shared memory, so there is one launch, no workspace, no atomic and a fixed order -- the
+// result is bit-reproducible.  The top k <= 32 are kept sorted over the 32 lanes of a warp as 64-bit keys
+// (order-preserving value bits, then the complement of the index: equal logits go to the lowest
+// index); a vector is looked at only if its largest element reaches the warp's k-th best.
+//
+// Backward: reads the logits, writes the gradient; one exponential per element.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "forge_host.h"
+
+namespace cg = cooperative_groups;
+
+namespace forge {
+namespace loss {
+
+constexpr int THREADS = 512;
+constexpr int WARPS = THREADS / 32;
+constexpr int MAX_CLUSTER = 16;
+constexpr int MAX_TOP = 32;
+constexpr float LAZY_LOG = 6.0f;        // e^6 = 403: far from fp32's range even times the largest vocabulary
+constexpr float LOG2E = 1.44269504088896340736f;
+
+struct Params {
+  const uint8_t* logits;
+  const long long* targets;
+  float* logprobs;
+  float* entropy;
+  float* lse;
+  float* top_logprobs;
+  long long* top_ids;
+  float* stats;                          // partial mode: (rows, 5) = m, S, T, target's z, target found
+  unsigned long long* keys;              // partial mode: (rows, top_k)
+  long long vocab, ld, ignore_index, vocab_start, vocab_total;
+  int top_k;
+  float inv_t;                           // 1 / temperature
+};
+
+struct Acc {
+  float m, s, t;                         // m in units of z
+};
+
+// a NaN stays a NaN (fmaxf would drop it)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (m, S, T) of two disjoint sets of columns -> of their union.  A set without a finite logit has m = -inf
+// and S = T = 0 (or NaN, if it holds a NaN): it must not enter the differences below.
+__device__ __forceinline__ Acc join(const Acc& a, const Acc& b) {
+  if (a.m == -INFINITY) return Acc{b.m, a.s + b.s, a.t + b.t};
+  if (b.m == -INFINITY) return Acc{a.m, a.s + b.s, a.t + b.t};
+  const float m = fmaxf(a.m, b.m);
+  const float da = a.m - m, db = b.m - m;
+  const float fa = exp2_approx(da * LOG2E), fb = exp2_approx(db * LOG2E);
+  // one of da, db is zero; the other may be so low that its factor is 0, and 0 * -inf would be NaN
+  const float ta = fa > 0.0f ? fa * (a.t + da * a.s) : 0.0f * a.s;
+  const float tb = fb > 0.0f ? fb * (b.t + db * b.s) : 0.0f * b.s;
+  return Acc{m, fa * a.s + fb * b.s, ta + tb};
+}
+
+__device__ __forceinline__ Acc warp_join(Acc a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Acc b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+    b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
+    // the lower lane's operand first in both lanes: the same bits everywhere
+    a = (threadIdx.x & o) ? join(b, a) : join(a, b);
+  }
+  return a;
+}
+
+// ----- sorted lists of 32 keys, one per lane, descending ------------------------------------------
+typedef unsigned long long u64;
+
+__device__ __forceinline__ u64 make_key(float x, uint32_t index) {
+  uint32_t u = __float_as_uint(x + 0.0f);             // -0 becomes +0: they are equal
+  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return (static_cast<u64>(u) << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ float key_value(u64 k) {
+  const uint32_t u = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+__device__ __forceinline__ uint32_t key_index(u64 k) { return 0xffffffffu - static_cast<uint32_t>(k); }
+
+// every lane offers one key (0: none); the list keeps the best 32, `floor` is its k-th entry
+__device__ __forceinline__ void warp_insert(u64& list, u64& floor, u64 key, int k, int lane) {
+  uint32_t mask;
+  while ((mask = __ballot_sync(0xffffffffu, key > floor)) != 0) {
+    const int src = __ffs(mask) - 1;
+    const u64 x = __shfl_sync(0xffffffffu, key, src);
+    const int pos = __popc(__ballot_sync(0xffffffffu, list > x));
+    const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
+    if (lane == pos) list = x;
+    else if (lane > pos) list = up;
+    floor = __shfl_sync(0xffffffffu, list, k - 1);
+    if (lane == src) key = 0;
+  }
+}
+
+// the best 32 of two descending lists, descending: the larger of a[i], b[31 - i] is a bitonic
+// sequence, five exchange steps sort it
+__device__ __forceinline__ u64 warp_merge(u64 a, u64 b, int lane) {
+  const u64 r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  u64 c = a > r ? a : r;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const u64 d = __shfl_xor_sync(0xffffffffu, c, o);
+    c = (((lane & o) == 0) == (c > d)) ? c : d;
+  }
+  return c;
+}
+
+// ----- one thread's running sums ------------------------------------------------------------------
+struct Run {
+  float m, thr;                          // m in raw logit units; rescale when a value exceeds thr
+  float2 s, t;                           // two interleaved partial sums; t in raw logit units
+};
+
+__device__ __forceinline__ void rebase(Run& r, float vmax, float lazy, float c) {
+  if (r.m != -INFINITY) {
+    const float d = r.m - vmax;
+    const float f = exp2_approx(d * c);
+    const float df = f > 0.0f ? d : 0.0f;
+    r.t.x = f * (r.t.x + df * r.s.x);
+    r.t.y = f * (r.t.y + df * r.s.y);
+    r.s.x *= f;
+    r.s.y *= f;
+  }
+  r.m = vmax;
+  r.thr = vmax + lazy;
+}
+
+template <int N>
+__device__ __forceinline__ void accumulate(Run& r, const float (&x)[N], float vmax, float lazy, float c) {
+  if (vmax > r.thr) rebase(r, vmax, lazy, c);
+  const float nm = r.m == -INFINITY ? 0.0f : -r.m;
+  float2 t = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 z = fadd2(make_float2(x[i], x[i + 1]), make_float2(nm, nm));
+    const float2 y = fmul2(z, make_float2(c, c));
+    const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+    r.s = fadd2(r.s, e);
+    t = ffma2(e, z, t);
+  }
+  const float tt = t.x + t.y;
+  if (tt != tt) {
+    // a masked (-inf) logit gave 0 * -inf: take its product as zero; a NaN stays one
+    t = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float z = max_nan(x[i] + nm, -3.0e38f);
+      t.x = __fmaf_rn(exp2_approx(z * c), z, t.x);
+    }
+  }
+  r.t = fadd2(r.t, t);
+}
+
+template <int DT>
+struct Vec;
+template <>
+struct Vec<DT_BF16> {
+  static constexpr int N = 8, ES = 2;
+  static __device__ __forceinline__ float unpack(const uint4& q, float (&x)[8]) {
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+    __nv_bfloat162 mx = *reinterpret_cast<const __nv_bfloat162*>(&u[0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      if (i > 0) mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&u[i]));
+    }
+    return fmaxf(__low2float(mx), __high2float(mx));
+  }
+  static __device__ __forceinline__ float one(const uint8_t* p) {
+    return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16);
+  }
+};
+template <>
+struct Vec<DT_F32> {
+  static constexpr int N = 4, ES = 4;
+  static __device__ __forceinline__ float unpack(const uint4& q, float (&x)[4]) {
+    x[0] = __uint_as_float(q.x); x[1] = __uint_as_float(q.y);
+    x[2] = __uint_as_float(q.z); x[3] = __uint_as_float(q.w);
+    return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  }
+  static __device__ __forceinline__ float one(const uint8_t* p) { return *reinterpret_cast<const float*>(p); }
+};
+
+__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
+  uint4 q;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+               : "l"(p));
+  return q;
+}
+
+struct Shared {
+  Acc warp_acc[WARPS];
+  u64 warp_keys[WARPS][32];
+  Acc cta_acc[MAX_CLUSTER];              // written by the cluster's CTAs into the first one's copy
+  u64 cta_keys[MAX_CLUSTER][32];
+};
+
+// what the joined row comes to; `keys` of warp 0's lanes
+__device__ __forceinline__ void write_row(const Params& p, long long row, const Acc& a, float zt, bool found, bool top,
+                                          u64 list, int lane) {
+  const float log_s = logf(a.s);
+  if (lane == 0) {
+    const long long t = p.targets ? p.targets[row] : p.ignore_index;
+    const bool ignored = p.targets == nullptr || t == p.ignore_index;
+    if (p.logprobs) p.logprobs[row] = ignored ? 0.0f : (found ? (zt - a.m) - log_s : NAN);
+    if (p.entropy) p.entropy[row] = log_s - a.t / a.s;
+    if (p.lse) p.lse[row] = a.m + log_s;
+  }
+  if (top && lane < p.top_k) {
+    p.top_ids[row * p.top_k + lane] = static_cast<long long>(key_index(list));
+    p.top_logprobs[row * p.top_k + lane] = (key_value(list) * p.inv_t - a.m) - log_s;
+  }
+}
+
+template <int DT, bool TOP>
+__global__ void __launch_bounds__(THREADS) logprobs_kernel(const Params p, const int cs) {
+  using V = Vec<DT>;
+  constexpr int N = V::N, ES = V::ES;
+  __shared__ Shared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = blockIdx.x / cs;
+  const int rank = blockIdx.x % cs;
+  const uint8_t* base = p.logits + row * p.ld * ES;
+  if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+
+  // columns: `head` up to the first 16-byte boundary, nv whole vectors shared out over the cluster, a tail
+  const int mis = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / ES;
+  const long long head = mis < p.vocab ? mis : p.vocab;
+  const long long nv = (p.vocab - head) / N;
+  const long long tail0 = head + nv * N;
+  const uint8_t* vbase = base + head * ES;
+  // whole warps of vectors per CTA
+  const long long per = ((nv + cs - 1) / cs + 31) / 32 * 32;
+  const long long v_begin = rank * per < nv ? rank * per : nv;
+  const long long v_end = v_begin + per < nv ? v_begin + per : nv;
+
+  const float c = p.inv_t * LOG2E;
+  const float lazy = LAZY_LOG / p.inv_t;
+  Run r;
+  r.m = -INFINITY;
+  r.thr = -INFINITY;
+  r.s = r.t = make_float2(0.0f, 0.0f);
+  u64 list = 0, floor_key = 0;
+  float floor_val = -INFINITY;           // the k-th best value so far (-inf: the list is not full)
+
+  auto offer = [&](const float* x, int n, float vmax, long long first, bool live) {
+    if constexpr (TOP) {
+      if (__any_sync(0xffffffffu, live && vmax >= floor_val)) {
+        for (int i = 0; i < n; ++i) {
+          const u64 key = live ? make_key(x[i], static_cast<uint32_t>(p.vocab_start + first + i)) : 0;
+          warp_insert(list, floor_key, key, p.top_k, lane);
+        }
+        floor_val = floor_key != 0 ? key_value(floor_key) : -INFINITY;
+      }
+    }
+  };
+
+  constexpr int U = 4;
+  long long v = v_begin + warp * 32;
+  for (; v + (U - 1) * THREADS + 32 <= v_end; v += U * THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = load_stream(vbase + (v + u * THREADS + lane) * 16);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[N];
+      const float vmax = V::unpack(q[u], x);
+      accumulate<N>(r, x, vmax, lazy, c);
+      offer(x, N, vmax, head + (v + u * THREADS + lane) * N, true);
+    }
+  }
+  for (; v < v_end; v += THREADS) {
+    const bool live = v + lane < v_end;
+    float x[N];
+    float vmax = -INFINITY;
+    if (live) {
+      vmax = V::unpack(load_stream(vbase + (v + lane) * 16), x);
+      accumulate<N>(r, x, vmax, lazy, c);
+    }
+    offer(x, N, vmax, head + (v + lane) * N, live);
+  }
+  // at most N - 1 single columns at either end: warp 0 of the first CTA, one per lane
+  if (rank == 0 && warp == 0) {
+    const int n_tail = static_cast<int>(p.vocab - tail0);
+    const int n_one = static_cast<int>(head) + n_tail;
+    const bool live = lane < n_one;
+    const long long col = lane < head ? lane : tail0 + (lane - head);
+    float x[2] = {-INFINITY, -INFINITY};
+    if (live) {
+      x[0] = V::one(base + col * ES);
+      accumulate<2>(r, x, x[0], lazy, c);
+    }
+    offer(x, 1, x[0], col, live);
+  }
+
+  // raw units -> units of z
+  Acc a{r.m == -INFINITY ? r.m : r.m * p.inv_t, r.s.x + r.s.y, (r.t.x + r.t.y) * p.inv_t};
+  a = warp_join(a);
+  if (lane == 0) sh.warp_acc[warp] = a;
+  if constexpr (TOP) sh.warp_keys[warp][lane] = list;
+  __syncthreads();
+  if (warp == 0) {
+    a = warp_join(lane < WARPS ? sh.warp_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
+    if constexpr (TOP) {
+      for (int w = 1; w < WARPS; ++w) list = warp_merge(list, sh.warp_keys[w][lane], lane);
+    }
+  }
+  if (cs > 1) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");       // the first CTA has started
+    cg::cluster_group cluster = cg::this_cluster();
+    if (warp == 0) {
+      Shared* first = cluster.map_shared_rank(&sh, 0);
+      if (lane == 0) first->cta_acc[rank] = a;
+      if constexpr (TOP) first->cta_keys[rank][lane] = list;
+    }
+    cluster.sync();
+    if (rank == 0 && warp == 0) {
+      a = warp_join(lane < cs ? sh.cta_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
+      if constexpr (TOP) {
+        for (int w = 1; w < cs; ++w) list = warp_merge(list, sh.cta_keys[w][lane], lane);
+      }
+    }
+  }
+  if (rank != 0 || warp != 0) return;
+
+  // the given token: one load by every lane of the warp
+  const long long t = p.targets ? p.targets[row] : p.ignore_index;
+  const long long tl = t - p.vocab_start;
+  const bool found = t != p.ignore_index && t >= 0 && t < p.vocab_total && tl >= 0 && tl < p.vocab;
+  const float zt = found ? V::one(base + tl * ES) * p.inv_t : 0.0f;
+  if (p.stats != nullptr) {
+    if (lane == 0) {
+      float* s = p.stats + row * 5;
+      s[0] = a.m; s[1] = a.s; s[2] = a.t; s[3] = zt; s[4] = found ? 1.0f : 0.0f;
+    }
+    if (TOP && lane < p.top_k) p.keys[row * p.top_k + lane] = list;
+  } else {
+    write_row(p, row, a, zt, found, TOP, list, lane);
+  }
+}
+
+// Partial results of `parts` slices of the vocabulary (stats (parts, rows, 5), keys (parts, rows, k)) ->
+// the rows' results.  One warp per row.
+__global__ void __launch_bounds__(256) logprobs_join_kernel(const Params p, const float* stats, const u64* keys, int parts,
+                                                            long long rows) {
+  const int lane = threadIdx.x & 31;
+  const long long row = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  Acc a{-INFINITY, 0.0f, 0.0f};
+  float zt = 0.0f;
+  bool found = false;
+  u64 list = 0;
+  for (int q = 0; q < parts; ++q) {
+    const float* s = stats + (q * rows + row) * 5;
+    a = join(a, Acc{s[0], s[1], s[2]});
+    if (s[4] != 0.0f) { zt = s[3]; found = true; }
+    if (p.top_k > 0) list = warp_merge(list, lane < p.top_k ? keys[(q * rows + row) * p.top_k + lane] : 0, lane);
+  }
+  write_row(p, row, a, zt, found, p.top_k > 0, list, lane);
+}
+
+struct BackParams {
+  const uint8_t* logits;
+  uint8_t* grad;
+  const long long* targets;
+  const float* lse;
+  const float* entropy;
+  const float* g_logprob;
+  const float* g_entropy;
+  long long vocab, ld, ld_grad, ignore_index, vocab_start, vocab_total;
+  float inv_t;
+};
+
+template <int DT>
+__device__ __forceinline__ uint4 pack(const float* x);
+template <>
+__device__ __forceinline__ uint4 pack<DT_BF16>(const float* x) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+template <>
+__device__ __forceinline__ uint4 pack<DT_F32>(const float* x) {
+  return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+template <int DT>
+__device__ __forceinline__ void store_one(uint8_t* p, float x) {
+  if constexpr (DT == DT_BF16) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(float_to_bf16_bits(x));
+  else *reinterpret_cast<float*>(p) = x;
+}
+
+constexpr int BACK_THREADS = 256;
+
+// grid: (column chunks, rows folded over y and z)
+template <int DT, bool ENT>
+__global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const BackParams p, long long rows, int vec_per_cta) {
+  using V = Vec<DT>;
+  constexpr int N = V::N, ES = V::ES;
+  const long long row = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
+  if (row >= rows) return;
+  const uint8_t* in = p.logits + row * p.ld * ES;
+  uint8_t* out = p.grad + row * p.ld_grad * ES;
+  const long long t = p.targets ? p.targets[row] : p.ignore_index;
+  const bool ignored = t == p.ignore_index;
+  const float gl = (ignored || p.g_logprob == nullptr) ? 0.0f
+                   : (t < 0 || t >= p.vocab_total)     ? NAN
+                                                       : p.g_logprob[row] * p.inv_t;
+  const float c = p.inv_t * LOG2E;
+  const float nl = -p.lse[row] * LOG2E;                  // log2 p = x c + nl
+  const float gh = ENT ? p.g_entropy[row] * p.inv_t : 0.0f;
+  // dx = p (-gl - gh (log p + H)) + gl [j = t] = p (a + b log2 p) + ...
+  const float a = ENT ? -gl - gh * p.entropy[row] : -gl;
+  const float b = ENT ? -gh / LOG2E : 0.0f;
+  const long long tl = t - p.vocab_start;                // column of the target, if it is one of these
+  const bool here = !ignored && tl >= 0 && tl < p.vocab;
+  auto one = [&](float x) {
+    const float y = __fmaf_rn(x, c, nl);
+    const float pr = exp2_approx(y);
+    if constexpr (ENT) return pr * __fmaf_rn(b, max_nan(y, -3.0e38f), a);
+    else return pr * a;
+  };
+  const int mis = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / ES;
+  const bool wide = (reinterpret_cast<uintptr_t>(in) & 15) == (reinterpret_cast<uintptr_t>(out) & 15);
+  const long long head = mis < p.vocab ? mis : p.vocab;
+  const long long nv = (p.vocab - head) / N;
+  const long long v_begin = static_cast<long long>(blockIdx.x) * vec_per_cta;
+  const long long v_end = v_begin + vec_per_cta < nv ? v_begin + vec_per_cta : nv;
+  constexpr int U = 4;
+  for (long long v = v_begin + threadIdx.x; v < v_end; v += U * BACK_THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v + u * BACK_THREADS < v_end) q[u] = load_stream(in + (head + (v + u * BACK_THREADS) * N) * ES);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long vv = v + u * BACK_THREADS;
+      if (vv >= v_end) break;
+      float x[N];
+      V::unpack(q[u], x);
+      const long long col = head + vv * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = one(x[i]);
+      if (here && tl >= col && tl < col + N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (tl == col + i) x[i] += gl;
+      }
+      if (wide) {
+        *reinterpret_cast<uint4*>(out + col * ES) = pack<DT>(x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) store_one<DT>(out + (col + i) * ES, x[i]);
+      }
+    }
+  }
+  if (blockIdx.x == 0) {
+    const long long tail0 = head + nv * N;
+    const int n_one = static_cast<int>(head + (p.vocab - tail0));
+    const int i = threadIdx.x;
+    if (i < n_one) {
+      const long long col = i < head ? i : tail0 + (i - head);
+      float x = one(V::one(in + col * ES));
+      if (here && tl == col) x += gl;
+      store_one<DT>(out + col * ES, x);
+    }
+  }
+}
+
+static int check(const ForgeLogprobsArgs& a, const char* what) {
+  if (a.rows < 0 || a.vocab < 0) return fail(FORGE_ERR_INVALID_ARG, "%s: negative dimension", what);
+  if (a.dtype != FORGE_DT_BF16 && a.dtype != FORGE_DT_F32) return fail(FORGE_ERR_INVALID_ARG, "%s: unknown dtype %d", what, a.dtype);
+  if (a.top_k < 0 || a.top_k > MAX_TOP) return fail(FORGE_ERR_INVALID_ARG, "%s: top_k must be 0 .. %d (got %d)", what, MAX_TOP, a.top_k);
+  if (!(a.temperature > 0.0) || !isfinite(a.temperature) || !isfinite(1.0f / static_cast<float>(a.temperature)) ||
+      static_cast<float>(a.temperature) == 0.0f)
+    return fail(FORGE_ERR_INVALID_ARG, "%s: temperature must be a positive finite number (got %g)", what, a.temperature);
+  if (a.vocab_start < 0 || a.vocab_total < a.vocab_start + a.vocab || a.vocab_total > 0x7fffffffll)
+    return fail(FORGE_ERR_SHAPE, "%s: columns [%lld, %lld) of a vocabulary of %lld", what, (long long)a.vocab_start,
+                (long long)(a.vocab_start + a.vocab), (long long)a.vocab_total);
+  if (a.top_k > a.vocab_total) return fail(FORGE_ERR_SHAPE, "%s: top_k (%d) exceeds the vocabulary (%lld)", what, a.top_k, (long long)a.vocab_total);
+  if (a.rows > 0 && (a.vocab < 1 || a.ld < a.vocab)) return fail(FORGE_ERR_SHAPE, "%s: vocab=%lld ld=%lld", what, (long long)a.vocab, (long long)a.ld);
+  if (a.rows * MAX_CLUSTER > 0x7fffffffll) return fail(FORGE_ERR_SHAPE, "%s: %lld rows", what, (long long)a.rows);
+  return FORGE_OK;
+}
+
+static Params make_params(const ForgeLogprobsArgs& a) {
+  Params p;
+  p.logits = static_cast<const uint8_t*>(a.logits);
+  p.targets = reinterpret_cast<const long long*>(a.targets);
+  p.logprobs = a.logprobs; p.entropy = a.entropy; p.lse = a.lse;
+  p.top_logprobs = a.top_logprobs; p.top_ids = reinterpret_cast<long long*>(a.top_ids);
+  p.stats = a.stats; p.keys = reinterpret_cast<u64*>(a.keys);
+  p.vocab = a.vocab; p.ld = a.ld; p.ignore_index = a.ignore_index;
+  p.vocab_start = a.vocab_start; p.vocab_total = a.vocab_total;
+  p.top_k = a.top_k;
+  p.inv_t = static_cast<float>(1.0 / a.temperature);
+  return p;
+}
+
+template <int DT, bool TOP>
+static int launch_forward(const Params& p, long long rows, int cs, cudaStream_t stream) {
+  auto* fn = logprobs_kernel<DT, TOP>;
+  if (cs > 8) {
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "logprobs: cluster attribute: %s", cudaGetErrorString(e));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * cs));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cs;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fn, p, cs);
+  if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "logprobs launch: %s", cudaGetErrorString(e));
+  return FORGE_OK;
+}
+
+}  // namespace loss
+}  // namespace forge
+
+using namespace forge;
+
+extern "C" int forge_logprobs_forward(const ForgeLogprobsArgs* args, void* cuda_stream) {
+  if (args == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_forward: args is NULL");
+  const ForgeLogprobsArgs& a = *args;
+  int rc = loss::check(a, "forge_logprobs_forward");
+  if (rc != FORGE_OK) return rc;
+  if (a.rows == 0) return FORGE_OK;
+  if (a.logits == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_forward: logits is NULL");
+  const int es = a.dtype == FORGE_DT_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(a.logits) % es != 0) return fail(FORGE_ERR_ALIGNMENT, "forge_logprobs_forward: logits are not element-aligned");
+  if (a.stats == nullptr && a.vocab != a.vocab_total)
+    return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_forward: a slice of the vocabulary needs `stats`");
+  if (a.top_k > 0 && (a.stats != nullptr ? a.keys == nullptr : (a.top_logprobs == nullptr || a.top_ids == nullptr)))
+    return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_forward: top_k without its outputs");
+  const DeviceInfo* di = current_device_info();
+  if (di == nullptr) return FORGE_ERR_CUDA;
+  if (di->cc_major != 10) return fail(FORGE_ERR_DEVICE, "device %d is sm_%d%d, not sm_100", di->device, di->cc_major, di->cc_minor);
+  // A row is cut over as many CTAs as keep the GPU's CTA slots (four of 512 threads per SM) filled, while each
+  // still has a batch of vectors per thread to load.
+  const long long slots = 4ll * di->sm_count;
+  const long long vecs = a.vocab * es / 16;
+  int cs = 1;
+  while (cs < loss::MAX_CLUSTER && a.rows * cs * 2 <= slots && vecs > static_cast<long long>(cs) * loss::THREADS) cs *= 2;
+  const loss::Params p = loss::make_params(a);
+  cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (a.dtype == FORGE_DT_BF16)
+    return a.top_k > 0 ? loss::launch_forward<DT_BF16, true>(p, a.rows, cs, s) : loss::launch_forward<DT_BF16, false>(p, a.rows, cs, s);
+  return a.top_k > 0 ? loss::launch_forward<DT_F32, true>(p, a.rows, cs, s) : loss::launch_forward<DT_F32, false>(p, a.rows, cs, s);
+}
+
+extern "C" int forge_logprobs_join(const ForgeLogprobsArgs* args, const float* stats, const uint64_t* keys, int32_t parts,
+                                   void* cuda_stream) {
+  if (args == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_join: args is NULL");
+  ForgeLogprobsArgs a = *args;
+  a.vocab_start = 0;                       // the joined rows cover the whole vocabulary
+  a.vocab = a.vocab_total;
+  a.ld = a.vocab_total;
+  int rc = loss::check(a, "forge_logprobs_join");
+  if (rc != FORGE_OK) return rc;
+  if (parts < 1) return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_join: parts = %d", parts);
+  if (a.rows == 0) return FORGE_OK;
+  if (stats == nullptr || (a.top_k > 0 && (keys == nullptr || a.top_logprobs == nullptr || a.top_ids == nullptr)))
+    return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_join: null pointer");
+  const loss::Params p = loss::make_params(a);
+  loss::logprobs_join_kernel<<<static_cast<unsigned>((a.rows + 7) / 8), 256, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
+      p, stats, reinterpret_cast<const loss::u64*>(keys), parts, a.rows);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "logprobs join launch: %s", cudaGetErrorString(e));
+  return FORGE_OK;
+}
+
+extern "C" int forge_logprobs_backward(const ForgeLogprobsArgs* args, const float* g_logprob, const float* g_entropy, void* grad,
+                                       int64_t ld_grad, void* cuda_stream) {
+  if (args == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_backward: args is NULL");
+  const ForgeLogprobsArgs& a = *args;
+  int rc = loss::check(a, "forge_logprobs_backward");
+  if (rc != FORGE_OK) return rc;
+  if (a.rows == 0) return FORGE_OK;
+  if (a.logits == nullptr || a.lse == nullptr || grad == nullptr || (g_entropy != nullptr && a.entropy == nullptr))
+    return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_backward: null pointer");
+  if (ld_grad < a.vocab) return fail(FORGE_ERR_SHAPE, "forge_logprobs_backward: ld_grad=%lld", (long long)ld_grad);
+  const int es = a.dtype == FORGE_DT_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(a.logits) % es != 0 || reinterpret_cast<uintptr_t>(grad) % es != 0)
+    return fail(FORGE_ERR_ALIGNMENT, "forge_logprobs_backward: tensors are not element-aligned");
+  loss::BackParams p;
+  p.logits = static_cast<const uint8_t*>(a.logits);
+  p.grad = static_cast<uint8_t*>(grad);
+  p.targets = reinterpret_cast<const long long*>(a.targets);
+  p.lse = a.lse; p.entropy = a.entropy; p.g_logprob = g_logprob; p.g_entropy = g_entropy;
+  p.vocab = a.vocab; p.ld = a.ld; p.ld_grad = ld_grad; p.ignore_index = a.ignore_index;
+  p.vocab_start = a.vocab_start; p.vocab_total = a.vocab_total;
+  p.inv_t = static_cast<float>(1.0 / a.temperature);
+  // 16 KB of logits per CTA (four 16-byte loads per thread)
+  const int vec_per_cta = loss::BACK_THREADS * 4;
+  const long long vecs = a.vocab * es / 16;
+  const long long chunks = std::max<long long>(1, (vecs + vec_per_cta - 1) / vec_per_cta);
+  const unsigned gy = static_cast<unsigned>(std::min<int64_t>(a.rows, 32768));
+  const unsigned gz = static_cast<unsigned>((a.rows + gy - 1) / gy);
+  if (gz > 65535u) return fail(FORGE_ERR_SHAPE, "forge_logprobs_backward: %lld rows", (long long)a.rows);
+  const dim3 grid(static_cast<unsigned>(chunks), gy, gz);
+  cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (a.dtype == FORGE_DT_BF16) {
+    if (g_entropy) loss::logprobs_backward_kernel<DT_BF16, true><<<grid, loss::BACK_THREADS, 0, s>>>(p, a.rows, vec_per_cta);
+    else loss::logprobs_backward_kernel<DT_BF16, false><<<grid, loss::BACK_THREADS, 0, s>>>(p, a.rows, vec_per_cta);
+  } else {
+    if (g_entropy) loss::logprobs_backward_kernel<DT_F32, true><<<grid, loss::BACK_THREADS, 0, s>>>(p, a.rows, vec_per_cta);
+    else loss::logprobs_backward_kernel<DT_F32, false><<<grid, loss::BACK_THREADS, 0, s>>>(p, a.rows, vec_per_cta);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "logprobs backward launch: %s", cudaGetErrorString(e));
+  return FORGE_OK;
+}

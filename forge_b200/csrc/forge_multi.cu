@@ -1,0 +1,512 @@
+// One AdamW step over a list of tensors of any sizes, and the common norm of a list of gradients.
+//
+// The tensors' pointers and sizes travel in the kernel's parameter block (up to MAX_TENSORS per launch),
+// so a step is one launch, needs no descriptor in device memory and can be captured as it is.  The
+// elements of all tensors are cut into chunks; a CTA finds its tensor by bisection of the chunks' prefix
+// sums.  A thread owns 8 consecutive elements, so eight lanes own a quantisation block of 64 and agree on
+// its absmax with three shuffles; the blocks run over a tensor's elements in memory order, which for a
+// (V, H) weight with H % 64 == 0 is the layout of the fused path.  Same per-element arithmetic as the fused
+// path (forge_update.cuh).
+//
+// Bound by memory: 3 element sizes of the parameter (read, write, gradient) and 2 of each moment.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "forge_host.h"
+
+namespace forge {
+namespace multi {
+
+constexpr int THREADS = 256;
+constexpr int EPT = 8;                          // elements per thread and pass
+constexpr int PASS = THREADS * EPT;             // 2048 elements
+constexpr int MAX_TENSORS = 448;
+
+struct Item {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  long long n;
+};
+
+template <int CAP>
+struct Params {
+  Item item[CAP];
+  int first_chunk[CAP + 1];                     // first chunk of each tensor; [count] = number of chunks
+  int count;
+  int passes;                                   // a chunk is this many passes of PASS elements
+  const float* coef;                            // gradients are multiplied by *coef, if given
+  const Hyper* hyper_device;
+  Hyper hyper;
+};
+
+// largest i with first[i] <= c
+__device__ __forceinline__ int find_tensor(const int* first, int count, int c) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= c) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* base, long long i, float (&x)[8]) {
+  if constexpr (DT == DT_F32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
+    const float4 a = q[0], b = q[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[2 * k] = __uint_as_float(u[k] << 16);
+      x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store8(void* base, long long i, const float (&x)[8]) {
+  if constexpr (DT == DT_F32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
+    q[0] = make_float4(x[0], x[1], x[2], x[3]);
+    q[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = float_to_bf16_bits(x[2 * k]) | (float_to_bf16_bits(x[2 * k + 1]) << 16);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + i) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float load1(const void* base, long long i) {
+  if constexpr (DT == DT_F32) return static_cast<const float*>(base)[i];
+  else return bf16_bits_to_float(static_cast<const uint16_t*>(base)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void store1(void* base, long long i, float x) {
+  if constexpr (DT == DT_F32) static_cast<float*>(base)[i] = x;
+  else static_cast<uint16_t*>(base)[i] = static_cast<uint16_t>(float_to_bf16_bits(x));
+}
+
+__device__ __forceinline__ bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+template <int W_DT, int G_DT, int ST, int CAP>
+__global__ void __launch_bounds__(THREADS) multi_adamw_kernel(const __grid_constant__ Params<CAP> p) {
+  constexpr bool QUANT = ST == ST_INT8 || ST == ST_FP8_BLOCK;
+  constexpr int S_DT = ST == ST_F32 ? DT_F32 : DT_BF16;
+  const int chunk = blockIdx.x;
+  const int ti = find_tensor(p.first_chunk, p.count, chunk);
+  const Item it = p.item[ti];
+  const Hyper hy = p.hyper_device != nullptr ? *p.hyper_device : p.hyper;
+  const float coef = p.coef != nullptr ? *p.coef : 1.0f;
+  const long long begin = static_cast<long long>(chunk - p.first_chunk[ti]) * p.passes * PASS;
+  const bool wide = aligned(it.p, 16) && aligned(it.g, 16) && aligned(it.m, QUANT ? 8 : 16) && aligned(it.v, QUANT ? 8 : 16);
+
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const long long i0 = begin + static_cast<long long>(pass) * PASS + threadIdx.x * EPT;
+    // whole warps leave together (the block absmax is agreed on by shuffles)
+    if (i0 - (threadIdx.x & 31) * EPT >= it.n) break;
+    const long long left = it.n - i0;
+    const int live = left >= EPT ? EPT : (left > 0 ? static_cast<int>(left) : 0);
+    const bool vec = wide && live == EPT;
+    float w[EPT], g[EPT], m[EPT], v[EPT];
+    uint32_t mq[2] = {0, 0}, vq[2] = {0, 0};
+    float sm = 1.0f, sv = 1.0f;
+    if (vec) {
+      load8<G_DT>(it.g, i0, g);
+      load8<W_DT>(it.p, i0, w);
+      if constexpr (QUANT) {
+        const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(it.m) + i0);
+        const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(it.v) + i0);
+        mq[0] = a.x; mq[1] = a.y; vq[0] = b.x; vq[1] = b.y;
+      } else {
+        load8<S_DT>(it.m, i0, m);
+        load8<S_DT>(it.v, i0, v);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) {
+        const bool on = k < live;
+        g[k] = on ? load1<G_DT>(it.g, i0 + k) : 0.0f;
+        w[k] = on ? load1<W_DT>(it.p, i0 + k) : 0.0f;
+        if constexpr (QUANT) {
+          if (on) {
+            mq[k >> 2] |= static_cast<uint32_t>(static_cast<const uint8_t*>(it.m)[i0 + k]) << (8 * (k & 3));
+            vq[k >> 2] |= static_cast<uint32_t>(static_cast<const uint8_t*>(it.v)[i0 + k]) << (8 * (k & 3));
+          }
+        } else {
+          m[k] = on ? load1<S_DT>(it.m, i0 + k) : 0.0f;
+          v[k] = on ? load1<S_DT>(it.v, i0 + k) : 0.0f;
+        }
+      }
+    }
+    if constexpr (QUANT) {
+      if (live > 0) {
+        sm = it.m_scale[i0 >> 6];
+        sv = it.v_scale[i0 >> 6];
+      }
+      if constexpr (ST == ST_INT8) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { mq[j] ^= 0x80808080u; vq[j] ^= 0x80808080u; }
+      }
+#pragma unroll
+      for (int k = 0; k < EPT; k += 2) {
+        float2 m2, v2;
+        if constexpr (ST == ST_INT8) {
+          m2 = int8x2_to_float(mq[k >> 2], k & 3);
+          v2 = int8x2_to_float(vq[k >> 2], k & 3);
+        } else {
+          e4m3x2_to_float(mq[k >> 2] >> (8 * (k & 3)), m2.x, m2.y);
+          e4m3x2_to_float(vq[k >> 2] >> (8 * (k & 3)), v2.x, v2.y);
+        }
+        m2 = fmul2(m2, make_float2(sm, sm));
+        v2 = fmul2(v2, make_float2(sv, sv));
+        m[k] = m2.x; m[k + 1] = m2.y;
+        v[k] = fmaxf(v2.x, 1e-8f); v[k + 1] = fmaxf(v2.y, 1e-8f);
+      }
+    }
+    if (p.coef != nullptr) {
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) g[k] = f_mul(g[k], coef);
+    }
+#pragma unroll
+    for (int k = 0; k < EPT; k += 2) {
+      float2 m2 = make_float2(m[k], m[k + 1]), v2 = make_float2(v[k], v[k + 1]);
+      const float2 w2 = adamw_update2(make_float2(w[k], w[k + 1]), make_float2(g[k], g[k + 1]), m2, v2, hy);
+      w[k] = w2.x; w[k + 1] = w2.y;
+      m[k] = m2.x; m[k + 1] = m2.y;
+      v[k] = v2.x; v[k + 1] = v2.y;
+    }
+    uint32_t mo[2], vo[2];
+    if constexpr (QUANT) {
+      float am = 0.0f, av = 0.0f;
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) {
+        // elements past the end of the tensor take no part in the last block's absmax
+        am = fmaxf(am, k < live ? fabsf(m[k]) : 0.0f);
+        av = fmaxf(av, k < live ? fabsf(v[k]) : 0.0f);
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+        av = fmaxf(av, __shfl_xor_sync(0xffffffffu, av, o));
+      }
+      const float sm_new = ST == ST_INT8 ? int8_scale(am) : fp8blk_scale(am);
+      const float sv_new = ST == ST_INT8 ? int8_scale(av) : fp8blk_scale(av);
+      const float rsm = f_rcp(sm_new), rsv = f_rcp(sv_new);
+      const float2 nsm2 = make_float2(-sm_new, -sm_new), nsv2 = make_float2(-sv_new, -sv_new);
+      const float2 rsm2 = make_float2(rsm, rsm), rsv2 = make_float2(rsv, rsv);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int k = 4 * j;
+        const float2 qm01 = div2_by_rcp(make_float2(m[k], m[k + 1]), nsm2, rsm2);
+        const float2 qm23 = div2_by_rcp(make_float2(m[k + 2], m[k + 3]), nsm2, rsm2);
+        const float2 qv01 = div2_by_rcp(make_float2(v[k], v[k + 1]), nsv2, rsv2);
+        const float2 qv23 = div2_by_rcp(make_float2(v[k + 2], v[k + 3]), nsv2, rsv2);
+        if constexpr (ST == ST_INT8) {
+          mo[j] = int8x4_pack(int8x2_round(qm01), int8x2_round(qm23));
+          vo[j] = int8x4_pack(int8x2_round(qv01), int8x2_round(qv23));
+        } else {
+          mo[j] = e4m3x2_code_bits(qm01.x, qm01.y) | (e4m3x2_code_bits(qm23.x, qm23.y) << 16);
+          vo[j] = e4m3x2_code_bits(qv01.x, qv01.y) | (e4m3x2_code_bits(qv23.x, qv23.y) << 16);
+        }
+      }
+      if (live > 0 && (i0 & 63) == 0) {
+        it.m_scale[i0 >> 6] = sm_new;
+        it.v_scale[i0 >> 6] = sv_new;
+      }
+    }
+    if (vec) {
+      store8<W_DT>(it.p, i0, w);
+      if constexpr (QUANT) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(it.m) + i0) = make_uint2(mo[0], mo[1]);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(it.v) + i0) = make_uint2(vo[0], vo[1]);
+      } else {
+        store8<S_DT>(it.m, i0, m);
+        store8<S_DT>(it.v, i0, v);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) {
+        if (k >= live) continue;
+        store1<W_DT>(it.p, i0 + k, w[k]);
+        if constexpr (QUANT) {
+          static_cast<uint8_t*>(it.m)[i0 + k] = static_cast<uint8_t>(mo[k >> 2] >> (8 * (k & 3)));
+          static_cast<uint8_t*>(it.v)[i0 + k] = static_cast<uint8_t>(vo[k >> 2] >> (8 * (k & 3)));
+        } else {
+          store1<S_DT>(it.m, i0 + k, m[k]);
+          store1<S_DT>(it.v, i0 + k, v[k]);
+        }
+      }
+    }
+  }
+}
+
+// ----- common norm --------------------------------------------------------------------------------
+struct NormItem {
+  const void* g;
+  long long n;
+};
+template <int CAP>
+struct NormParams {
+  NormItem item[CAP];
+  int first_chunk[CAP + 1];
+  int count;
+  int passes;
+  double* partial;                              // one sum per CTA of the launch
+};
+
+__device__ __forceinline__ double block_sum_d(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = 0.0;
+  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) t += red[i];
+  return t;
+}
+
+// squares are summed eight at a time in fp32 and from there on in fp64, in an order that does not
+// depend on the run
+template <int DT, int CAP>
+__global__ void __launch_bounds__(THREADS) multi_norm_kernel(const __grid_constant__ NormParams<CAP> p) {
+  __shared__ double red[THREADS / 32];
+  const int chunk = blockIdx.x;
+  const int ti = find_tensor(p.first_chunk, p.count, chunk);
+  const NormItem it = p.item[ti];
+  const long long begin = static_cast<long long>(chunk - p.first_chunk[ti]) * p.passes * PASS;
+  const bool wide = aligned(it.g, 16);
+  double sum = 0.0;
+#pragma unroll 4
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const long long i0 = begin + static_cast<long long>(pass) * PASS + threadIdx.x * EPT;
+    if (i0 >= it.n) break;
+    float x[EPT];
+    if (wide && i0 + EPT <= it.n) {
+      load8<DT>(it.g, i0, x);
+    } else {
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) x[k] = i0 + k < it.n ? load1<DT>(it.g, i0 + k) : 0.0f;
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < EPT; ++k) s = __fmaf_rn(x[k], x[k], s);
+    sum += static_cast<double>(s);
+  }
+  const double t = block_sum_d(sum, red);
+  if (threadIdx.x == 0) p.partial[blockIdx.x] = t;
+}
+
+// norm = sqrt of the partial sums; coef = min(1, max_norm / (norm + 1e-6))
+__global__ void __launch_bounds__(1024) multi_norm_final_kernel(const double* partial, int n, float max_norm, float* norm, float* coef) {
+  __shared__ double red[32];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
+  s = block_sum_d(s, red);
+  if (threadIdx.x == 0) {
+    const float r = static_cast<float>(sqrt(s));
+    *norm = r;
+    if (coef != nullptr) {
+      const float q = max_norm / (r + 1e-6f);
+      *coef = q > 1.0f ? 1.0f : q;              // a NaN stays one
+    }
+  }
+}
+
+// A chunk is as many passes as leave about eight CTAs for each of an SM's eight slots: enough to even out
+// the ends of a launch, few enough that looking the tensor up costs nothing.
+static int pick_passes(long long total, int sm_count) {
+  const long long want = total / (static_cast<long long>(PASS) * sm_count * 64);
+  return static_cast<int>(std::max<long long>(1, std::min<long long>(want, 8)));
+}
+static long long chunks_of(long long n, int passes) { return (n + static_cast<long long>(PASS) * passes - 1) / (static_cast<long long>(PASS) * passes); }
+
+static constexpr long long MAX_CHUNKS = 0x7fffffffll;
+
+template <int W_DT, int G_DT, int ST, int CAP>
+static int launch_adamw(const ForgeMultiItem* const* items, int count, int passes, const ForgeMultiArgs& a, cudaStream_t stream) {
+  Params<CAP> p;
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    const ForgeMultiItem& s = *items[i];
+    p.item[i] = Item{s.param, s.grad, s.m, s.v, s.m_scale, s.v_scale, static_cast<long long>(s.numel)};
+    p.first_chunk[i] = static_cast<int>(chunks);
+    chunks += chunks_of(s.numel, passes);
+  }
+  if (chunks > MAX_CHUNKS) return fail(FORGE_ERR_SHAPE, "forge_multi_adamw: too many elements for one launch");
+  p.first_chunk[count] = static_cast<int>(chunks);
+  p.count = count;
+  p.passes = passes;
+  p.coef = a.grad_coef;
+  p.hyper_device = static_cast<const Hyper*>(a.hyper_device);
+  p.hyper = make_hyper(a.hyper);
+  multi_adamw_kernel<W_DT, G_DT, ST, CAP><<<static_cast<unsigned>(chunks), THREADS, 0, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "multi-tensor AdamW launch: %s", cudaGetErrorString(e));
+  return FORGE_OK;
+}
+
+template <int W_DT, int G_DT, int CAP>
+static int by_state(const ForgeMultiItem* const* items, int count, int passes, const ForgeMultiArgs& a, cudaStream_t s) {
+  switch (a.state_mode) {
+    case FORGE_ST_F32: return launch_adamw<W_DT, G_DT, ST_F32, CAP>(items, count, passes, a, s);
+    case FORGE_ST_BF16: return launch_adamw<W_DT, G_DT, ST_BF16, CAP>(items, count, passes, a, s);
+    case FORGE_ST_INT8: return launch_adamw<W_DT, G_DT, ST_INT8, CAP>(items, count, passes, a, s);
+    case FORGE_ST_FP8_BLOCK: return launch_adamw<W_DT, G_DT, ST_FP8_BLOCK, CAP>(items, count, passes, a, s);
+  }
+  return fail(FORGE_ERR_UNSUPPORTED, "forge_multi_adamw: state mode %d is not built", a.state_mode);
+}
+
+template <int CAP>
+static int by_types(int w, int g, const ForgeMultiItem* const* items, int count, int passes, const ForgeMultiArgs& a, cudaStream_t s) {
+  if (w == FORGE_DT_BF16) return g == FORGE_DT_BF16 ? by_state<DT_BF16, DT_BF16, CAP>(items, count, passes, a, s) : by_state<DT_BF16, DT_F32, CAP>(items, count, passes, a, s);
+  return g == FORGE_DT_BF16 ? by_state<DT_F32, DT_BF16, CAP>(items, count, passes, a, s) : by_state<DT_F32, DT_F32, CAP>(items, count, passes, a, s);
+}
+
+template <int DT>
+static int launch_norm(const ForgeNormItem* const* items, int count, int passes, double* partial, long long* used, cudaStream_t stream) {
+  NormParams<MAX_TENSORS> p;
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    p.item[i] = NormItem{items[i]->grad, static_cast<long long>(items[i]->numel)};
+    p.first_chunk[i] = static_cast<int>(chunks);
+    chunks += chunks_of(items[i]->numel, passes);
+  }
+  p.first_chunk[count] = static_cast<int>(chunks);
+  p.count = count;
+  p.passes = passes;
+  p.partial = partial;
+  multi_norm_kernel<DT, MAX_TENSORS><<<static_cast<unsigned>(chunks), THREADS, 0, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "multi-tensor norm launch: %s", cudaGetErrorString(e));
+  *used = chunks;
+  return FORGE_OK;
+}
+
+static bool dtype_ok(int d) { return d == FORGE_DT_BF16 || d == FORGE_DT_F32; }
+
+}  // namespace multi
+}  // namespace forge
+
+using namespace forge;
+
+extern "C" int forge_multi_adamw(const ForgeMultiArgs* args, void* cuda_stream) {
+  if (args == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_multi_adamw: args is NULL");
+  const ForgeMultiArgs& a = *args;
+  if (a.count < 0 || (a.count > 0 && a.items == nullptr)) return fail(FORGE_ERR_INVALID_ARG, "forge_multi_adamw: bad item list");
+  if (a.state_mode != FORGE_ST_F32 && a.state_mode != FORGE_ST_BF16 && a.state_mode != FORGE_ST_INT8 && a.state_mode != FORGE_ST_FP8_BLOCK)
+    return fail(FORGE_ERR_UNSUPPORTED, "forge_multi_adamw: state mode %d is not built", a.state_mode);
+  if (a.hyper_device == nullptr && a.hyper.step < 1) return fail(FORGE_ERR_INVALID_ARG, "step must be >= 1 (got %d)", a.hyper.step);
+  const bool quant = a.state_mode == FORGE_ST_INT8 || a.state_mode == FORGE_ST_FP8_BLOCK;
+  const int ses = a.state_mode == FORGE_ST_F32 ? 4 : (a.state_mode == FORGE_ST_BF16 ? 2 : 1);
+  long long total = 0;
+  for (int i = 0; i < a.count; ++i) {
+    const ForgeMultiItem& s = a.items[i];
+    if (s.numel < 0) return fail(FORGE_ERR_INVALID_ARG, "forge_multi_adamw: tensor %d has %lld elements", i, (long long)s.numel);
+    if (!multi::dtype_ok(s.param_dtype) || !multi::dtype_ok(s.grad_dtype))
+      return fail(FORGE_ERR_INVALID_ARG, "forge_multi_adamw: tensor %d has an unknown dtype", i);
+    if (s.numel == 0) continue;
+    if (s.param == nullptr || s.grad == nullptr || s.m == nullptr || s.v == nullptr || (quant && (s.m_scale == nullptr || s.v_scale == nullptr)))
+      return fail(FORGE_ERR_INVALID_ARG, "forge_multi_adamw: tensor %d has a null pointer", i);
+    if (reinterpret_cast<uintptr_t>(s.param) % (s.param_dtype == FORGE_DT_BF16 ? 2 : 4) || reinterpret_cast<uintptr_t>(s.grad) % (s.grad_dtype == FORGE_DT_BF16 ? 2 : 4) ||
+        reinterpret_cast<uintptr_t>(s.m) % ses || reinterpret_cast<uintptr_t>(s.v) % ses)
+      return fail(FORGE_ERR_ALIGNMENT, "forge_multi_adamw: tensor %d is not element-aligned", i);
+    total += s.numel;
+  }
+  if (total == 0) return FORGE_OK;
+  const DeviceInfo* di = current_device_info();
+  if (di == nullptr) return FORGE_ERR_CUDA;
+  const int passes = multi::pick_passes(total, di->sm_count);
+  if (total / multi::PASS + a.count > multi::MAX_CHUNKS) return fail(FORGE_ERR_SHAPE, "forge_multi_adamw: %lld elements", total);
+  // one launch per combination of types and MAX_TENSORS tensors
+  std::vector<const ForgeMultiItem*> list;
+  try {
+    list.reserve(a.count);
+  } catch (...) {
+    return fail(FORGE_ERR_INVALID_ARG, "forge_multi_adamw: out of host memory");
+  }
+  for (int combo = 0; combo < 4; ++combo) {
+    const int w = combo & 1, g = combo >> 1;
+    list.clear();
+    for (int i = 0; i < a.count; ++i)
+      if (a.items[i].numel > 0 && a.items[i].param_dtype == w && a.items[i].grad_dtype == g) list.push_back(&a.items[i]);
+    for (size_t i = 0; i < list.size(); i += multi::MAX_TENSORS) {
+      const int n = static_cast<int>(std::min<size_t>(multi::MAX_TENSORS, list.size() - i));
+      const int rc = multi::by_types<multi::MAX_TENSORS>(w, g, list.data() + i, n, passes, a, static_cast<cudaStream_t>(cuda_stream));
+      if (rc != FORGE_OK) return rc;
+    }
+  }
+  return FORGE_OK;
+}
+
+static long long norm_total(const ForgeNormItem* items, int32_t count) {
+  long long total = 0;
+  for (int i = 0; i < count; ++i) total += items[i].numel > 0 ? items[i].numel : 0;
+  return total;
+}
+
+// a chunk of the norm is 1 .. 64 passes long, so that there are never many partial sums
+static int norm_passes(long long total) {
+  return static_cast<int>(std::max<long long>(1, std::min<long long>(64, total / (static_cast<long long>(multi::PASS) * 148 * 8))));
+}
+
+extern "C" size_t forge_multi_norm_scratch_bytes(const ForgeNormItem* items, int32_t count) {
+  if (items == nullptr || count <= 0) return 0;
+  const int passes = norm_passes(norm_total(items, count));
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) chunks += items[i].numel > 0 ? multi::chunks_of(items[i].numel, passes) : 0;
+  return static_cast<size_t>(chunks) * sizeof(double);
+}
+
+extern "C" int forge_multi_norm(const ForgeNormItem* items, int32_t count, double max_norm, float* norm, float* coef, void* scratch,
+                                size_t scratch_bytes, void* cuda_stream) {
+  if (count < 0 || (count > 0 && items == nullptr) || norm == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_multi_norm: null pointer");
+  if (coef != nullptr && !(max_norm > 0.0)) return fail(FORGE_ERR_INVALID_ARG, "forge_multi_norm: max_norm must be positive (got %g)", max_norm);
+  for (int i = 0; i < count; ++i) {
+    if (items[i].numel < 0 || !multi::dtype_ok(items[i].dtype) || (items[i].numel > 0 && items[i].grad == nullptr))
+      return fail(FORGE_ERR_INVALID_ARG, "forge_multi_norm: bad tensor %d", i);
+    if (reinterpret_cast<uintptr_t>(items[i].grad) % (items[i].dtype == FORGE_DT_BF16 ? 2 : 4))
+      return fail(FORGE_ERR_ALIGNMENT, "forge_multi_norm: tensor %d is not element-aligned", i);
+  }
+  const size_t need = forge_multi_norm_scratch_bytes(items, count);
+  if (need > scratch_bytes || (need > 0 && scratch == nullptr))
+    return fail(FORGE_ERR_SCRATCH, "forge_multi_norm needs %zu bytes of scratch (got %zu)", need, scratch_bytes);
+  if (reinterpret_cast<uintptr_t>(scratch) % sizeof(double)) return fail(FORGE_ERR_ALIGNMENT, "forge_multi_norm: scratch is not 8-byte aligned");
+  if (need / sizeof(double) > static_cast<size_t>(multi::MAX_CHUNKS)) return fail(FORGE_ERR_SHAPE, "forge_multi_norm: too many elements");
+  const int passes = norm_passes(norm_total(items, count));
+  double* partial = static_cast<double*>(scratch);
+  long long used = 0;
+  std::vector<const ForgeNormItem*> list;
+  try {
+    list.reserve(count);
+  } catch (...) {
+    return fail(FORGE_ERR_INVALID_ARG, "forge_multi_norm: out of host memory");
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  for (int dt = 0; dt < 2; ++dt) {
+    list.clear();
+    for (int i = 0; i < count; ++i)
+      if (items[i].numel > 0 && items[i].dtype == dt) list.push_back(&items[i]);
+    for (size_t i = 0; i < list.size(); i += multi::MAX_TENSORS) {
+      const int n = static_cast<int>(std::min<size_t>(multi::MAX_TENSORS, list.size() - i));
+      long long chunks = 0;
+      const int rc = dt == FORGE_DT_BF16 ? multi::launch_norm<DT_BF16>(list.data() + i, n, passes, partial + used, &chunks, s)
+                                         : multi::launch_norm<DT_F32>(list.data() + i, n, passes, partial + used, &chunks, s);
+      if (rc != FORGE_OK) return rc;
+      used += chunks;
+    }
+  }
+  multi::multi_norm_final_kernel<<<1, 1024, 0, s>>>(partial, static_cast<int>(used), static_cast<float>(max_norm), norm, coef);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "multi-tensor norm launch: %s", cudaGetErrorString(e));
+  return FORGE_OK;
+}

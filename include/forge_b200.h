@@ -313,6 +313,127 @@ int forge_rmsnorm_backward(const void* x, const void* gamma, const void* grad_y,
                            void* cuda_stream);
 size_t forge_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t H);
 
+/* ---- the loss at the logits ----------------------------------------------------------------------
+ * No counterpart in the reference (its examples use the model's own cross entropy).
+ *
+ * Rows of logits x (rows, vocab), row-major with pitch `ld` elements, bf16 or fp32; z = x / temperature.
+ *   logprobs[r] = z[t] - log sum_j e^z[j] for the given token t = targets[r]; 0 where t == ignore_index, NaN
+ *                 where t is outside [0, vocab_total) (nothing is read there)
+ *   entropy[r]  = -sum_j p_j log p_j,   lse[r] = log sum_j e^z[j]
+ *   top_logprobs / top_ids (rows, top_k): the top_k <= 32 largest logits' log probabilities and columns, in
+ *                 descending order, equal logits by ascending column
+ * A logit of -inf has probability zero; a row of nothing else, or with a NaN or +inf, gives NaN as the
+ * formulas do (its top_ids are then valid columns in no particular order).  All sums are fp32.
+ *
+ * Vocabulary slices (a row-sharded lm_head): the logits are columns [vocab_start, vocab_start + vocab) of
+ * vocab_total; with `stats` non-NULL the forward writes stats (rows, 5) and keys (rows, top_k) instead of
+ * results, and forge_logprobs_join turns the `parts` slices' stats (parts, rows, 5) and keys (parts, rows,
+ * top_k) into the results. */
+typedef struct ForgeLogprobsArgs {
+  const void* logits;
+  const int64_t* targets;    /* NULL: every row is ignored (entropy and alternatives only)              */
+  int64_t rows, vocab, ld;
+  int64_t vocab_start, vocab_total;
+  int64_t ignore_index;
+  double temperature;
+  int32_t dtype;             /* FORGE_DT_* of logits (and of the gradient)                              */
+  int32_t top_k;
+  float* logprobs;           /* (rows,); outputs may be NULL except those of top_k                      */
+  float* entropy;            /* (rows,)                                                                 */
+  float* lse;                /* (rows,)                                                                 */
+  float* top_logprobs;
+  int64_t* top_ids;
+  float* stats;
+  uint64_t* keys;
+} ForgeLogprobsArgs;
+int forge_logprobs_forward(const ForgeLogprobsArgs* args, void* cuda_stream);
+int forge_logprobs_join(const ForgeLogprobsArgs* args, const float* stats, const uint64_t* keys, int32_t parts,
+                        void* cuda_stream);
+
+/* grad[r, j] = (g_logprob[r] (1[j = t] - p_j) - g_entropy[r] p_j (log p_j + entropy[r])) / temperature, in the
+ * logits' type, row pitch ld_grad.  args: as in the forward, with `lse` (and `entropy`, if g_entropy is given)
+ * as it wrote them; the logits of a slice give the slice's columns of the gradient.  g_logprob, g_entropy:
+ * (rows,) or NULL for zero. */
+int forge_logprobs_backward(const ForgeLogprobsArgs* args, const float* g_logprob, const float* g_entropy, void* grad,
+                            int64_t ld_grad, void* cuda_stream);
+
+/* ---- AdamW over a list of tensors -----------------------------------------------------------------
+ * forge_optimizer_update for every tensor of a list (the parameters that are not fused linears: embeddings,
+ * norms, biases) in one launch per combination of types and 448 tensors.  Tensors are contiguous, of any
+ * size and alignment; the moments follow `state_mode` (F32, BF16, INT8, FP8_BLOCK), the scales of the 8-bit
+ * modes belong to 64 consecutive elements each (ceil(numel / 64) of them; the last block may be short), which
+ * for a (V, H) weight with H % 64 == 0 is the layout of ForgeState.  The reference leaves these parameters to
+ * torch.optim (src/fused_grad_optimizer/module.py:218-222).  Tensors must not overlap. */
+typedef struct ForgeMultiItem {
+  void* param;
+  const void* grad;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  int64_t numel;
+  int32_t param_dtype, grad_dtype;
+} ForgeMultiItem;
+typedef struct ForgeMultiArgs {
+  const ForgeMultiItem* items;
+  int32_t count;
+  int32_t state_mode;
+  ForgeHyper hyper;
+  const void* hyper_device;  /* as in ForgeWgradArgs, or NULL                                           */
+  const float* grad_coef;    /* device scalar every gradient is multiplied by, or NULL                  */
+} ForgeMultiArgs;
+int forge_multi_adamw(const ForgeMultiArgs* args, void* cuda_stream);
+
+/* norm = sqrt of the sum of the squares of all elements of a list of gradients, and, if `coef` is given,
+ * coef = min(1, max_norm / (norm + 1e-6)) (the factor of torch.nn.utils.clip_grad_norm_); both device
+ * scalars.  Sums are fp64 from eight elements up, in a fixed order.  scratch: 8-byte aligned. */
+typedef struct ForgeNormItem {
+  const void* grad;
+  int64_t numel;
+  int32_t dtype;
+  int32_t reserved;
+} ForgeNormItem;
+size_t forge_multi_norm_scratch_bytes(const ForgeNormItem* items, int32_t count);
+int forge_multi_norm(const ForgeNormItem* items, int32_t count, double max_norm, float* norm, float* coef, void* scratch,
+                     size_t scratch_bytes, void* cuda_stream);
+
+/* ---- products in 8-bit floating point ---------------------------------------------------------------
+ * forge_fp8_quantize: x (rows, cols) bf16 or fp32 -> e4m3 codes (row pitch ld_codes) and fp32 scales, one per
+ * block of block_rows x 128 (block_rows 1 or 128), scales (ceil(rows / block_rows), ceil(cols / 128))
+ * contiguous: scale = absmax / 448 + 1e-12, code = e4m3(x / scale) (the rule of FORGE_ST_FP8_BLOCK).  With
+ * 128 x 128 blocks also, if codes_t is given, the transposed codes (cols, rows) and scales.  An infinity makes its
+ * whole block NaN, a NaN only itself.  The reference has no counterpart (its fp8-operand experiments are not part
+ * of this library). */
+typedef struct ForgeFp8QuantizeArgs {
+  const void* x;
+  int64_t rows, cols, ld_x;
+  int32_t dtype, block_rows;
+  void* codes;
+  int64_t ld_codes;
+  float* scales;
+  void* codes_t;             /* or NULL */
+  int64_t ld_codes_t;
+  float* scales_t;
+} ForgeFp8QuantizeArgs;
+int forge_fp8_quantize(const ForgeFp8QuantizeArgs* args, void* cuda_stream);
+
+/* Y (M, N) bf16 = X W^T: X (M, K) codes with a scale per (row, 128 columns), W (N, K) codes with a scale per
+ * 128 x 128 block; the scales may have any strides (in elements).  Products of 128 terms are formed by the tensor
+ * cores and added in fp32, in an order that depends on the sizes alone.  Codes start on 16-byte boundaries with row
+ * pitches that are multiples of 16; K itself may be anything. */
+typedef struct ForgeFp8ProductArgs {
+  const void* x_codes;
+  const float* x_scales;
+  const void* w_codes;
+  const float* w_scales;
+  void* y;
+  int64_t M, N, K;
+  int64_t ld_x, ld_w, ld_y;
+  int64_t x_scale_row, x_scale_col, w_scale_row, w_scale_col;
+  int32_t* status;
+} ForgeFp8ProductArgs;
+int forge_fp8_product(const ForgeFp8ProductArgs* args, void* cuda_stream);
+
 /* Bytes of optimizer state the allocator must provide for a (V, H) parameter: the moment arrays
  * and, separately, the scale arrays (src/fused_grad_optimizer/state.py:95-130). */
 int forge_state_bytes(int32_t optimizer, int32_t mode, int64_t V, int64_t H, int32_t qblock,

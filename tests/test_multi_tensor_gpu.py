@@ -1,0 +1,324 @@
+"""AdamW over lists of tensors: moments, codes and scales bit for bit against the oracle, weights within its bar; the common
+norm against 64 bits; the optimizer class against the function, torch.optim and itself after a checkpoint."""
+
+import copy
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from forge_b200 import _lib
+from forge_b200 import kernel as K
+from forge_b200.multi_tensor import MultiTensorAdamW, multi_tensor_adamw, multi_tensor_grad_norm
+
+from tests.util import assert_bits_equal, assert_w_close, np32
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HP = dict(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, step=3)
+CODE = {"int8": torch.int8, "fp8_block": torch.float8_e4m3fn}
+
+
+def make(sizes, mode, pdt, gdt, seed=0, offset=0):
+    """CPU tensors of the given sizes and their CUDA copies; `offset` elements of misalignment for param and grad."""
+    g = torch.Generator().manual_seed(seed)
+
+    def dev(t):
+        if not offset:
+            return t.to(DEV)
+        big = torch.zeros(t.numel() + offset, dtype=t.dtype, device=DEV)
+        big[offset:] = t.reshape(-1).to(DEV)
+        return big[offset:].view(t.shape)
+
+    out = []
+    for n in sizes:
+        p = (torch.randn(n, generator=g) * 0.02).to(pdt)
+        gr = (torch.randn(n, generator=g) * 1e-2).to(gdt)
+        num = math.prod(n)
+        d = dict(p=p, g=gr)
+        if mode in CODE:
+            b = -(-num // 64)
+            if mode == "int8":
+                d["m"] = torch.randint(-127, 128, n, generator=g).to(torch.int8)
+                d["v"] = torch.randint(0, 128, n, generator=g).to(torch.int8)
+            else:
+                d["m"] = (torch.randn(n, generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+                d["v"] = (torch.randn(n, generator=g).abs() * 100).clamp(0, 448).to(torch.float8_e4m3fn)
+            d["ms"] = torch.rand(b, generator=g) * 1e-4 + 1e-6
+            d["vs"] = torch.rand(b, generator=g) * 1e-6 + 1e-8
+        else:
+            sdt = torch.float32 if mode == "f32" else torch.bfloat16
+            d["m"] = (torch.randn(n, generator=g) * 1e-3).to(sdt)
+            d["v"] = (torch.randn(n, generator=g).square() * 1e-5).to(sdt)
+        out.append((d, {k: dev(t) if k in "pgmv" else t.to(DEV) for k, t in d.items()}))
+    return out
+
+
+def call(items, mode, **kw):
+    quant = mode in CODE
+    return multi_tensor_adamw([d["p"] for d in items], [d["g"] for d in items], [d["m"] for d in items], [d["v"] for d in items],
+                              [d["ms"] for d in items] if quant else None, [d["vs"] for d in items] if quant else None,
+                              **{**HP, **kw})
+
+
+def expect(d, mode, coef=1.0):
+    """The oracle's step on one tensor, the last block filled up with zeros."""
+    h = oracle.Hyper(**HP)
+    n = d["p"].numel()
+    g = (d["g"].float() * coef).reshape(-1)
+    wb = d["p"].dtype == torch.bfloat16
+    if mode not in CODE:
+        w, m, v = np32(d["p"]).reshape(-1).copy(), np32(d["m"]).reshape(-1).copy(), np32(d["v"]).reshape(-1).copy()
+        oracle.adamw(w, m, v, np32(g), h, w_bf16=wb, s_bf16=mode == "bf16")
+        return dict(p=w, m=m, v=v)
+    b = -(-n // 64)
+
+    def pad(t, dt):
+        out = torch.zeros(b * 64, dtype=dt)
+        out[:n] = t.reshape(-1)
+        return np.ascontiguousarray(out.view(b, 64).numpy())
+
+    raw = torch.int8 if mode == "int8" else torch.uint8
+    w, gr = pad(d["p"].float(), torch.float32), pad(g, torch.float32)
+    m, v = pad(d["m"].view(raw), raw), pad(d["v"].view(raw), raw)
+    ms, vs = d["ms"].numpy().copy().reshape(b, 1), d["vs"].numpy().copy().reshape(b, 1)
+    oracle.adamw_blockq(w, m, v, ms, vs, gr, h, 64, w_bf16=wb, kind="int8" if mode == "int8" else "e4m3")
+    return dict(p=w.reshape(-1)[:n], m=m.reshape(-1)[:n], v=v.reshape(-1)[:n], ms=ms.reshape(-1), vs=vs.reshape(-1))
+
+
+def verify(pairs, mode, coef=1.0):
+    for i, (cpu, dev) in enumerate(pairs):
+        e = expect(cpu, mode, coef)
+        for k in ("m", "v"):
+            got = dev[k].reshape(-1)
+            assert_bits_equal(e[k], got.view(torch.uint8) if mode in CODE else got, f"tensor {i}: {k}")
+        if mode in CODE:
+            assert_bits_equal(e["ms"], dev["ms"], f"tensor {i}: m scale")
+            assert_bits_equal(e["vs"], dev["vs"], f"tensor {i}: v scale")
+        assert_w_close(e["p"], dev["p"].reshape(-1), cpu["p"].reshape(-1))
+
+
+SIZES = [(1,), (7,), (64,), (65, 3), (4096,), (130, 64), (5, 5, 5), (2049,), (40, 1025)]
+
+
+@pytest.mark.parametrize("mode", ["f32", "bf16", "int8", "fp8_block"])
+@pytest.mark.parametrize("pdt,gdt", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                     (torch.float32, torch.bfloat16), (torch.float32, torch.float32)])
+def test_against_the_oracle(mode, pdt, gdt):
+    pairs = make(SIZES, mode, pdt, gdt, seed=1)
+    call([d for _, d in pairs], mode)
+    verify(pairs, mode)
+
+
+@pytest.mark.parametrize("mode", ["f32", "int8"])
+@pytest.mark.parametrize("offset", [1, 3])
+def test_tensors_that_start_anywhere(mode, offset):
+    pairs = make(SIZES, mode, torch.bfloat16, torch.bfloat16, seed=2, offset=offset)
+    guard = [(d["p"]._base[:offset].clone(), d["p"]._base) for _, d in pairs]
+    call([d for _, d in pairs], mode)
+    verify(pairs, mode)
+    for before, base in guard:
+        assert torch.equal(before, base[:offset])
+
+
+def test_more_tensors_than_a_launch_holds_and_mixed_types():
+    sizes = [((i * 37) % 300 + 1,) for i in range(1000)]
+    pairs = make(sizes[:500], "f32", torch.bfloat16, torch.bfloat16, seed=3) + make(sizes[500:], "f32", torch.float32, torch.float32, seed=4)
+    order = torch.randperm(1000, generator=torch.Generator().manual_seed(5)).tolist()
+    pairs = [pairs[i] for i in order]
+    call([d for _, d in pairs], "f32")
+    verify(pairs, "f32")
+
+
+@pytest.mark.parametrize("mode", ["bf16", "int8", "fp8_block"])
+def test_equals_the_single_tensor_operator_bit_for_bit(mode):
+    (a, dev), = make([(2000, 512)], mode, torch.bfloat16, torch.bfloat16, seed=6)
+    one = {k: t.to(DEV) for k, t in a.items()}
+    call([dev], mode)
+    if mode == "bf16":
+        K.optimizer_only_adamw(one["g"], one["p"], one["m"], one["v"], **HP)
+    else:
+        fn = K.optimizer_only_adamw_int8state if mode == "int8" else K.optimizer_only_adamw_fp8block
+        fn(one["g"], one["p"], one["m"], one["v"], one["ms"].view(2000, 8), one["vs"].view(2000, 8), **HP)
+    for k in dev:
+        assert torch.equal(dev[k].view(torch.uint8), one[k].view(torch.uint8)), k
+
+
+def test_large_tensor_several_passes_per_chunk():
+    (cpu, dev), = make([(4001, 33000)], "int8", torch.bfloat16, torch.bfloat16, seed=7)
+    call([dev], "int8")
+    b = 64 * 1000
+    for lo in (0, 4001 * 33000 // 2 // 64 * 64, 4001 * 33000 // 64 * 64 - b):        # slices on block boundaries
+        hi = min(lo + b, 4001 * 33000)
+        cut = {k: (t.reshape(-1)[lo:hi] if k in "pgmv" else t[lo // 64:-(-hi // 64)]) for k, t in cpu.items()}
+        got = {k: (t.reshape(-1)[lo:hi] if k in "pgmv" else t[lo // 64:-(-hi // 64)]) for k, t in dev.items()}
+        verify([(cut, got)], "int8")
+
+
+@pytest.mark.parametrize("gdt", [torch.bfloat16, torch.float32])
+def test_norm_and_clipping(gdt):
+    pairs = make(SIZES + [(300000,)], "f32", torch.float32, gdt, seed=8)
+    grads = [d["g"] for _, d in pairs]
+    exact = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    norm, none = multi_tensor_grad_norm(grads)
+    # eight squares in fp32 (8 * 2^-24 of the sum), fp64 from there on, one rounding of the root
+    assert none is None and abs(float(norm) - exact) <= 1e-6 * exact
+    again, coef = multi_tensor_grad_norm(grads, 0.5 * exact)
+    assert torch.equal(norm, again) and abs(float(coef) - 0.5 * exact / (exact + 1e-6)) < 1e-6
+    assert float(multi_tensor_grad_norm(grads, 2 * exact)[1]) == 1.0
+    total = call([d for _, d in pairs], "f32", max_norm=0.5 * exact)
+    assert torch.equal(total, norm)
+    verify(pairs, "f32", coef.cpu())
+    assert float(multi_tensor_grad_norm([torch.zeros(5, device=DEV), torch.zeros(0, device=DEV)])[0]) == 0.0
+    assert float(multi_tensor_grad_norm([torch.zeros(0, device=DEV)])[0]) == 0.0
+    bad = torch.ones(100, device=DEV)
+    bad[3] = math.nan
+    n, c = multi_tensor_grad_norm([bad], 1.0)
+    assert n.isnan() and c.isnan()
+    bad[3] = math.inf
+    n, c = multi_tensor_grad_norm([bad], 1.0)
+    assert n.isinf() and c == 0
+
+
+def test_empty_and_expanded():
+    assert multi_tensor_adamw([], [], [], []) is None
+    pairs = make([(0,), (6, 4)], "f32", torch.float32, torch.float32, seed=9)
+    cpu, dev = pairs[1]
+    cpu["g"] = torch.full((1, 1), 0.25).expand(6, 4)
+    dev["g"] = torch.full((1, 1), 0.25, device=DEV).expand(6, 4)
+    call([d for _, d in pairs], "f32")
+    verify(pairs[1:], "f32")
+
+
+def test_device_hyper_stream_and_graph():
+    pairs = make(SIZES, "int8", torch.bfloat16, torch.bfloat16, seed=10)
+    devs = [d for _, d in pairs]
+    start = copy.deepcopy(devs)
+    hd = K.DeviceHyper(torch.device(DEV, 0))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            norm = call(devs, "int8", hyper_device=hd, max_norm=1e9)
+        for step in (1, 2):
+            hd.update(**{**HP, "step": step})
+            graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
+    for step in (1, 2):
+        want = call(start, "int8", step=step, max_norm=1e9)
+    assert torch.equal(norm, want)
+    for a, b in zip(devs, start):
+        for k in a:
+            assert torch.equal(a[k].view(torch.uint8), b[k].view(torch.uint8)), k
+
+
+def _params(seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter((torch.randn(n, generator=g) * 0.1).to(dtype).to(DEV)) for n in [(33, 64), (100,), (7,)]]
+
+
+def _give_grads(params, seed, skip=()):
+    g = torch.Generator().manual_seed(seed)
+    for i, p in enumerate(params):
+        gr = torch.randn(p.shape, generator=g).to(p.dtype).to(DEV)
+        p.grad = None if i in skip else gr
+
+
+def test_optimizer_class_follows_torch():
+    a, b = _params(1), _params(1)
+    mine = MultiTensorAdamW([{"params": a[:1]}, {"params": a[1:], "weight_decay": 0.0, "lr": 3e-3}], lr=1e-2, weight_decay=0.1,
+                            max_grad_norm=2.0)
+    ref = torch.optim.AdamW([{"params": b[:1]}, {"params": b[1:], "weight_decay": 0.0, "lr": 3e-3}], lr=1e-2, weight_decay=0.1)
+    for step in range(4):
+        skip = (1,) if step == 1 else ()             # one parameter sits a step out and counts its own steps
+        _give_grads(a, step, skip)
+        _give_grads(b, step, skip)
+        total = torch.nn.utils.clip_grad_norm_(b, 2.0)
+        mine.step()
+        ref.step()
+        assert abs(float(mine.last_grad_norm) - float(total)) < 1e-5 * float(total)
+    assert mine.state[a[1]]["step"] == 3 and mine.state[a[0]]["step"] == 4
+    for p, q in zip(a, b):
+        # a step moves a weight by about lr; the two evaluate it in fp32 with a few roundings each
+        assert (p - q).abs().max() < 4 * 1e-2 * 1e-5 + 1e-6
+
+
+@pytest.mark.parametrize("mode", ["f32", "bf16", "int8", "fp8_block"])
+def test_optimizer_checkpoint_continues_bit_for_bit(mode):
+    a, b = _params(2, torch.bfloat16), _params(2, torch.bfloat16)
+    opt = MultiTensorAdamW(a, lr=1e-2, state_mode=mode)
+    for step in range(2):
+        _give_grads(a, step)
+        opt.step()
+    for p, q in zip(b, a):
+        p.data.copy_(q.data)
+    other = MultiTensorAdamW(b, lr=5.0, state_mode=mode)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert other.param_groups[0]["lr"] == 1e-2
+    for p, q in zip(a, b):
+        for k, t in opt.state[p].items():
+            u = other.state[q][k]
+            assert (t == u) if k == "step" else (t.dtype == u.dtype and t.data_ptr() != u.data_ptr())
+    for o, ps in ((opt, a), (other, b)):
+        _give_grads(ps, 9)
+        o.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+        for k, t in opt.state[p].items():
+            u = other.state[q][k]
+            assert t == u if k == "step" else torch.equal(t.view(torch.uint8), u.view(torch.uint8))
+
+
+def test_optimizer_in_a_graph():
+    a, b = _params(3, torch.bfloat16), _params(3, torch.bfloat16)
+    opt, ref = MultiTensorAdamW(a, lr=1e-2, state_mode="int8"), MultiTensorAdamW(b, lr=1e-2, state_mode="int8")
+    _give_grads(a, 0)
+    _give_grads(b, 0)
+    opt.step()                                        # allocates the state
+    ref.step()
+    opt.enable_device_hyper()
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.pre_step()
+        with torch.cuda.graph(graph, stream=side):
+            opt.step()
+        graph.replay()
+        opt.param_groups[0]["lr"] = 2e-2
+        opt.pre_step()
+        graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
+    ref.step()
+    ref.param_groups[0]["lr"] = 2e-2
+    ref.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+
+
+def test_refusals():
+    p, g = torch.zeros(8, 8, device=DEV), torch.zeros(8, 8, device=DEV)
+    m, v = torch.zeros(8, 8, device=DEV), torch.zeros(8, 8, device=DEV)
+    ok = [p], [g], [m], [v]
+    q = torch.zeros(64, dtype=torch.int8, device=DEV)
+    s = torch.ones(1, device=DEV)
+    for args, kw in [(([p], [], [m], [v]), {}), (([p], [g[:4]], [m], [v]), {}), (([p], [g], [m[:4]], [v]), {}),
+                     (([p.half()], [g], [m], [v]), {}), (([p], [g.half()], [m], [v]), {}), (([p], [g], [m.half()], [v.half()]), {}),
+                     (([p], [g], [m], [v.bfloat16()]), {}), (([p.t()[:4]], [g[:4]], [m[:4]], [v[:4]]), {}),
+                     (([p], [g], [q], [q.clone()]), {}), (([p], [g], [q], [q.clone()], [s], [torch.ones(2, device=DEV)]), {}),
+                     (([p], [g], [q], [q.clone()], [s], [s.double()]), {}), (([p], [g], [m], [v], [s], [s]), {}),
+                     (([p, p], [g, g], [m, m.clone()], [v, v.clone()]), {}), (([p, p.clone()], [g, g], [m, m], [v, v.clone()]), {}),
+                     (([p], [g], [m], [m]), {}), (ok, dict(step=0)), (ok, dict(max_norm=0.0)), (ok, dict(max_norm=1.0, grad_coef=s)),
+                     (ok, dict(grad_coef=torch.ones(2, device=DEV)))]:
+        with pytest.raises(ValueError):
+            multi_tensor_adamw(*args, **kw)
+    with pytest.raises(_lib.ForgeLibraryError):
+        multi_tensor_adamw([p.cpu()], [g], [m], [v])
+    with pytest.raises(ValueError):
+        MultiTensorAdamW([torch.nn.Parameter(p)], state_mode="fp4")
+    with pytest.raises(ValueError):
+        MultiTensorAdamW([torch.nn.Parameter(p)], max_grad_norm=-1.0)
+    with pytest.raises(ValueError):
+        MultiTensorAdamW([torch.nn.Parameter(p)]).pre_step()
