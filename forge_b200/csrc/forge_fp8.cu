@@ -1,7 +1,7 @@
 // Products in 8-bit floating point with one fp32 scale for each block of 128, and the quantiser that
 // feeds them.
 //
-//   scale = absmax / 448 + 1e-12, code = e4m3(x / scale)   over 1 x 128 blocks of a row (activations,
+//   scale = absmax * fp32(1 / 448) + 1e-12, code = e4m3(x / scale)   over 1 x 128 blocks of a row (activations,
 //   gradients) or 128 x 128 blocks (weights; their transpose has the transposed scales)
 //   Y[m, n] = sum over kb of sx[m, kb] sw[n / 128, kb] * sum over the block's k of xq[m, k] wq[n, k]
 //
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
   float m = absmax8(x);
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float scale = fp8blk_scale(m);
+  const float scale = block_scale<448>(m);
   const uint2 c = codes8(x, scale, f_rcp(scale));
   uint8_t* dst = p.q + row * p.ld_q + col;
   if (live == 8 && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantParams 
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = fmaxf(m, red[i]);
-  const float scale = fp8blk_scale(m), rscale = f_rcp(scale);
+  const float scale = block_scale<448>(m), rscale = f_rcp(scale);
   uint2 c[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) {

@@ -6,7 +6,7 @@
 // sums.  A thread owns 8 consecutive elements, so eight lanes own a quantisation block of 64 and agree on
 // its absmax with three shuffles; the blocks run over a tensor's elements in memory order, which for a
 // (V, H) weight with H % 64 == 0 is the layout of the fused path.  Same per-element arithmetic as the fused
-// path (forge_update.cuh).
+// path (forge_update.cuh), but for the scales of the 8-bit moments (block_scale there: at most one ulp apart).
 //
 // Bound by memory: 3 element sizes of the parameter (read, write, gradient) and 2 of each moment.
 #include <cuda_bf16.h>
@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(THREADS) multi_adamw_kernel(const __grid_const
         am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
         av = fmaxf(av, __shfl_xor_sync(0xffffffffu, av, o));
       }
-      const float sm_new = ST == ST_INT8 ? int8_scale(am) : fp8blk_scale(am);
-      const float sv_new = ST == ST_INT8 ? int8_scale(av) : fp8blk_scale(av);
+      const float sm_new = block_scale<ST == ST_INT8 ? 127 : 448>(am);
+      const float sv_new = block_scale<ST == ST_INT8 ? 127 : 448>(av);
       const float rsm = f_rcp(sm_new), rsv = f_rcp(sv_new);
       const float2 nsm2 = make_float2(-sm_new, -sm_new), nsv2 = make_float2(-sv_new, -sv_new);
       const float2 rsm2 = make_float2(rsm, rsm), rsv2 = make_float2(rsv, rsv);

@@ -259,6 +259,13 @@ __device__ __forceinline__ void e5m2x2_to_float(uint32_t two_codes, float& lo, f
 __device__ __forceinline__ float fp8blk_scale(float absmax) {
   return f_add(div_by_const<448>(absmax), 1e-12f);
 }
+// The rule of the multi-tensor step and of the 8-bit products: absmax times the rounded reciprocal of the largest
+// code, one instruction instead of the corrected quotient above and at most one ulp from it.
+template <int TOP>
+__device__ __forceinline__ float block_scale(float absmax) {
+  constexpr float r = 1.0f / static_cast<float>(TOP);
+  return f_add(f_mul(absmax, r), 1e-12f);
+}
 __device__ __forceinline__ uint8_t e4m3_code(float x_scaled) {
   const float c = fminf(fmaxf(x_scaled, -448.0f), 448.0f);
   return static_cast<uint8_t>(__nv_cvt_float_to_fp8(c, __NV_SATFINITE, __NV_E4M3));

@@ -160,6 +160,8 @@ at::Tensor fused_linear(const at::Tensor& input, const at::Tensor& weight, const
 
 }  // namespace
 
+void bind_operators(pybind11::module_& m);   // forge_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "C++ autograd node of forge_b200.FusedLinear";
   pybind11::class_<NativeGroup, std::shared_ptr<NativeGroup>>(m, "Group")
@@ -189,4 +191,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_linear", &fused_linear, "Y = X W^T (+ b); the backward updates W in place through the C ABI");
   m.def("set_use_forge_dgrad", [](bool on) { g_use_forge_dgrad = on; });
   m.def("args_size", []() { return sizeof(ForgeWgradArgs); });
+  bind_operators(m);
 }

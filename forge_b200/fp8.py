@@ -16,11 +16,12 @@ import ctypes
 
 import torch
 
-from forge_b200 import _lib
+from forge_b200 import _lib, native
 from forge_b200.kernel import _require_cuda
 
 BLOCK = 128
 _CODE = torch.float8_e4m3fn
+_registered: set = set()      # devices whose status word the extension knows
 
 
 def _empty_codes(rows, cols, device):
@@ -43,10 +44,15 @@ def _pitch(t):
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1, transposed: bool = False, out=None):
     """e4m3 codes and fp32 scales of a bf16 or fp32 matrix ``x`` (R, C) in blocks of ``block_rows`` x 128 (1 or 128):
-    ``scale = absmax / 448 + 1e-12``, ``code = e4m3(x / scale)``.  Returns ``(codes (R, C), scales (ceil(R / block_rows),
+    ``scale = absmax * (1 / 448) + 1e-12``, ``code = e4m3(x / scale)`` in fp32.  Returns ``(codes (R, C), scales (ceil(R / block_rows),
     ceil(C / 128)))``; with ``transposed`` (128 x 128 blocks) also the codes (C, R) and scales of the transpose.  Code rows
     start on 16-byte boundaries.  An infinity makes its block NaN, a NaN only itself.  ``out``: tensors of an earlier call
     to write to."""
+    nat = native.module() if out is None else None
+    if nat is not None:
+        res = nat.fp8_quantize(x, block_rows, transposed)
+        if res is not None:
+            return res
     _require_cuda(x)
     _matrix(x, "x")
     if block_rows not in (1, BLOCK):
@@ -173,6 +179,15 @@ def _forward(x, bias, w):
 def fp8_linear(x: torch.Tensor, weight: Fp8Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x W^T (+ bias)`` with ``x`` (..., K) bf16 quantised by rows in the call; the input gradient is ``dY W`` with ``dY``
     quantised by rows in its turn, and needs the weight's transposed codes."""
+    nat = native.module() if bias is None else None
+    if nat is not None:
+        y = nat.fp8_linear(x, weight.codes, weight.scales, weight.codes_t, weight.scales_t)
+        if y is None and x.is_cuda and x.device.index not in _registered:
+            _registered.add(x.device.index)
+            nat.set_status_word(x.device.index, _lib.status_word(x.device).data_ptr())
+            y = nat.fp8_linear(x, weight.codes, weight.scales, weight.codes_t, weight.scales_t)
+        if y is not None:
+            return y
     _require_cuda(x, bias)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"fp8_linear takes bfloat16 activations (got {x.dtype})")

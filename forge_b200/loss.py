@@ -20,7 +20,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from forge_b200 import _lib
+from forge_b200 import _lib, native
 from forge_b200.kernel import _require_cuda
 
 MAX_TOP_K = 32
@@ -197,13 +197,20 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], *, top
     ``group``: the logits are this rank's columns ``[vocab_start, vocab_start + V)`` of ``vocab_total``, every rank of the
     process group calls with its own slice of the same rows (collective: two small all-gathers), and the results are the
     same on every rank.  The gradient is that of this rank's columns for the gradients that reach this rank's results."""
-    if temperature is None or not temperature > 0 or temperature == float("inf"):
+    temperature = float(temperature)
+    if not temperature > 0 or temperature == float("inf"):
         raise ValueError(f"temperature must be a positive finite number (got {temperature})")
-    if group is None and (vocab_start != 0 or (vocab_total is not None and vocab_total != logits.shape[-1])):
+    if group is None and (vocab_start != 0 or vocab_total is not None and vocab_total != logits.shape[-1]):
         raise ValueError("a slice of the vocabulary needs the process group of the other slices")
     if group is not None and vocab_total is None:
         raise ValueError("a slice of the vocabulary needs vocab_total")
+    if group is None:
+        nat = native.module()
+        if nat is not None:
+            out = nat.token_logprobs(logits, targets, top_k, temperature, ignore_index)
+            if out is not None:
+                return TokenLogprobs(*out)
     total = logits.shape[-1] if vocab_total is None else vocab_total
     _check(logits, targets, top_k, vocab_start, total)
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k, float(temperature), int(ignore_index), vocab_start, total,
+    return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k, temperature, int(ignore_index), vocab_start, total,
                                                group))

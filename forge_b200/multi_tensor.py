@@ -19,7 +19,7 @@ import ctypes
 
 import torch
 
-from forge_b200 import _lib
+from forge_b200 import _lib, native
 from forge_b200.kernel import DeviceHyper, _hyper, _require_cuda
 
 STATE_MODES = ("f32", "bf16", "int8", "fp8_block")
@@ -89,6 +89,13 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None
     ``max_norm``: multiply the gradients by ``min(1, max_norm / (norm + 1e-6))`` of their common norm, which is returned
     (an fp32 device scalar; None without ``max_norm``); ``grad_coef``: multiply them by a device scalar instead.
     ``hyper_device``: read lr, betas, eps, decay and step from a ``DeviceHyper`` block (for captured graphs)."""
+    nat = native.module()
+    if nat is not None and (max_norm is None or max_norm > 0):
+        out = nat.multi_adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, lr, beta1, beta2, eps,
+                              weight_decay, step, max_norm or 0.0, hyper_device.data_ptr() if hyper_device is not None else 0,
+                              grad_coef)
+        if out is not None:
+            return out[1]
     params, exp_avgs, exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)
     grads = _grads(grads)
     n = len(params)

@@ -362,7 +362,8 @@ int forge_logprobs_backward(const ForgeLogprobsArgs* args, const float* g_logpro
  * norms, biases) in one launch per combination of types and 448 tensors.  Tensors are contiguous, of any
  * size and alignment; the moments follow `state_mode` (F32, BF16, INT8, FP8_BLOCK), the scales of the 8-bit
  * modes belong to 64 consecutive elements each (ceil(numel / 64) of them; the last block may be short), which
- * for a (V, H) weight with H % 64 == 0 is the layout of ForgeState.  The reference leaves these parameters to
+ * for a (V, H) weight with H % 64 == 0 is the layout of ForgeState; scale = absmax * fp32(1 / 127 or 1 / 448) + 1e-12, at
+ * most one ulp from forge_optimizer_update's correctly rounded quotient.  The reference leaves these parameters to
  * torch.optim (src/fused_grad_optimizer/module.py:218-222).  Tensors must not overlap. */
 typedef struct ForgeMultiItem {
   void* param;
@@ -400,7 +401,7 @@ int forge_multi_norm(const ForgeNormItem* items, int32_t count, double max_norm,
 /* ---- products in 8-bit floating point ---------------------------------------------------------------
  * forge_fp8_quantize: x (rows, cols) bf16 or fp32 -> e4m3 codes (row pitch ld_codes) and fp32 scales, one per
  * block of block_rows x 128 (block_rows 1 or 128), scales (ceil(rows / block_rows), ceil(cols / 128))
- * contiguous: scale = absmax / 448 + 1e-12, code = e4m3(x / scale) (the rule of FORGE_ST_FP8_BLOCK).  With
+ * contiguous: scale = absmax * fp32(1 / 448) + 1e-12, code = e4m3(x / scale), each operation rounded once.  With
  * 128 x 128 blocks also, if codes_t is given, the transposed codes (cols, rows) and scales.  An infinity makes its
  * whole block NaN, a NaN only itself.  The reference has no counterpart (its fp8-operand experiments are not part
  * of this library). */
