@@ -10,9 +10,17 @@
 // in fp32).  The partial results of threads, warps and CTAs are joined by the same rule.  A row belongs
 // to a CLUSTER of CTAs (1 for many rows, up to 16 for a few): the join over a long row goes through
 // distributed shared memory, so there is one launch, no workspace, no atomic and a fixed order -- the
-// result is bit-reproducible.  The top k <= 32 are kept sorted over the 32 lanes of a warp as 64-bit keys
-// (order-preserving value bits, then the complement of the index: equal logits go to the lowest
-// index); a vector is looked at only if its largest element reaches the warp's k-th best.
+// result is bit-reproducible.
+//
+// The top k <= 32: keys of 64 bits (order-preserving value bits, then the complement of the index, so that
+// equal logits go to the lowest index) are collected in shared memory from elements that reach a bound T
+// below which the k-th best cannot lie, and ranked by counting: with n keys a thread reads n words to find its
+// key's place.  T first comes from the maxima of the threads' first vectors: of F full warps each has
+// ceil(k / F) lanes whose maximum is at least its ceil(k / F)-th largest, so the smallest of those is reached by k
+// elements at least; then it is the k-th best of what has been ranked, after 1, 4, 16, ... batches, so that about 3 k
+// elements pass in between.  Where too many pass (rows of ties, ascending rows), the CTA reads its columns once more
+// and every warp keeps a list of 32 that is sorted over its lanes.  Keeping such lists from the start took 69 us for 64
+// rows of 151936 fp32 logits with k = 20, nearly all of it in some hundred insertions per warp.
 //
 // Backward: reads the logits, writes the gradient; one exponential per element.
 #include <cooperative_groups.h>
@@ -20,6 +28,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "forge_host.h"
 
@@ -28,7 +37,7 @@ namespace cg = cooperative_groups;
 namespace forge {
 namespace loss {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 16;
 constexpr int MAX_TOP = 32;
@@ -80,17 +89,22 @@ __device__ __forceinline__ Acc join(const Acc& a, const Acc& b) {
   return Acc{m, fa * a.s + fb * b.s, ta + tb};
 }
 
-__device__ __forceinline__ Acc warp_join(Acc a) {
+// over the lanes of a warp: the maximum first, then plain sums
+__device__ __forceinline__ Acc warp_join(const Acc& a) {
+  float m = a.m, s = a.s, t = a.t;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (a.m != -INFINITY) {
+    const float d = a.m - m, f = exp2_approx(d * LOG2E);
+    t = f > 0.0f ? f * (t + d * s) : 0.0f * s;
+    s *= f;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    Acc b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-    // the lower lane's operand first in both lanes: the same bits everywhere
-    a = (threadIdx.x & o) ? join(b, a) : join(a, b);
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    t += __shfl_xor_sync(0xffffffffu, t, o);
   }
-  return a;
+  return Acc{m, s, t};
 }
 
 // ----- sorted lists of 32 keys, one per lane, descending ------------------------------------------
@@ -107,9 +121,30 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 __device__ __forceinline__ uint32_t key_index(u64 k) { return 0xffffffffu - static_cast<uint32_t>(k); }
 
+__device__ __forceinline__ u64 warp_merge(u64 a, u64 b, int lane);
+
+// the lanes' keys in descending order: a bitonic network
+__device__ __forceinline__ u64 warp_sort(u64 c, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const u64 d = __shfl_xor_sync(0xffffffffu, c, o);
+      const bool larger = ((lane & o) == 0) == ((lane & size) == 0);
+      c = (larger == (c > d)) ? c : d;
+    }
+  }
+  return c;
+}
+
 // every lane offers one key (0: none); the list keeps the best 32, `floor` is its k-th entry
-__device__ __forceinline__ void warp_insert(u64& list, u64& floor, u64 key, int k, int lane) {
-  uint32_t mask;
+__device__ __forceinline__ void warp_offer(u64& list, u64& floor, u64 key, int k, int lane) {
+  uint32_t mask = __ballot_sync(0xffffffffu, key > floor);
+  if (__popc(mask) > 4) {
+    list = warp_merge(list, warp_sort(key, lane), lane);
+    floor = __shfl_sync(0xffffffffu, list, k - 1);
+    return;
+  }
   while ((mask = __ballot_sync(0xffffffffu, key > floor)) != 0) {
     const int src = __ffs(mask) - 1;
     const u64 x = __shfl_sync(0xffffffffu, key, src);
@@ -138,6 +173,7 @@ __device__ __forceinline__ u64 warp_merge(u64 a, u64 b, int lane) {
 // ----- one thread's running sums ------------------------------------------------------------------
 struct Run {
   float m, thr;                          // m in raw logit units; rescale when a value exceeds thr
+  float nm;                              // -m, or 0 while there is no finite logit
   float2 s, t;                           // two interleaved partial sums; t in raw logit units
 };
 
@@ -152,33 +188,33 @@ __device__ __forceinline__ void rebase(Run& r, float vmax, float lazy, float c) 
     r.s.y *= f;
   }
   r.m = vmax;
+  r.nm = -vmax;
   r.thr = vmax + lazy;
 }
 
+// adds N logits whose masked (-inf) ones have been replaced by a finite number so low that its exponential is 0 and the
+// product in T stays 0
 template <int N>
-__device__ __forceinline__ void accumulate(Run& r, const float (&x)[N], float vmax, float lazy, float c) {
-  if (vmax > r.thr) rebase(r, vmax, lazy, c);
-  const float nm = r.m == -INFINITY ? 0.0f : -r.m;
-  float2 t = make_float2(0.0f, 0.0f);
+__device__ __forceinline__ void accumulate(Run& r, float2& t, const float (&x)[N], float c) {
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
-    const float2 z = fadd2(make_float2(x[i], x[i + 1]), make_float2(nm, nm));
+    const float2 z = fadd2(make_float2(x[i], x[i + 1]), make_float2(r.nm, r.nm));
     const float2 y = fmul2(z, make_float2(c, c));
     const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
     r.s = fadd2(r.s, e);
     t = ffma2(e, z, t);
   }
-  const float tt = t.x + t.y;
-  if (tt != tt) {
-    // a masked (-inf) logit gave 0 * -inf: take its product as zero; a NaN stays one
-    t = make_float2(0.0f, 0.0f);
+}
+// the same for logits as they are
+template <int N>
+__device__ __forceinline__ void accumulate_raw(Run& r, const float (&x)[N], float c) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float z = max_nan(x[i] + nm, -3.0e38f);
-      t.x = __fmaf_rn(exp2_approx(z * c), z, t.x);
-    }
+  for (int i = 0; i < N; ++i) {
+    const float z = x[i] + r.nm;
+    const float e = exp2_approx(z * c);
+    r.s.x += e;
+    r.t.x = __fmaf_rn(e, max_nan(z, -3.0e38f), r.t.x);
   }
-  r.t = fadd2(r.t, t);
 }
 
 template <int DT>
@@ -186,16 +222,27 @@ struct Vec;
 template <>
 struct Vec<DT_BF16> {
   static constexpr int N = 8, ES = 2;
-  static __device__ __forceinline__ float unpack(const uint4& q, float (&x)[8]) {
+  static __device__ __forceinline__ __nv_bfloat162 as2(uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); }
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[8]) {
     const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-    __nv_bfloat162 mx = *reinterpret_cast<const __nv_bfloat162*>(&u[0]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[2 * i] = __uint_as_float(u[i] << 16);
       x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      if (i > 0) mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&u[i]));
     }
-    return fmaxf(__low2float(mx), __high2float(mx));
+  }
+  // -inf -> the lowest finite number, two at a time (a NaN stays one)
+  static __device__ __forceinline__ uint4 unmask(const uint4& q) {
+    uint4 o;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.x) : "r"(q.x), "r"(0xff7fff7fu));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.y) : "r"(q.y), "r"(0xff7fff7fu));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.z) : "r"(q.z), "r"(0xff7fff7fu));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.w) : "r"(q.w), "r"(0xff7fff7fu));
+    return o;
+  }
+  static __device__ __forceinline__ float max_of(const uint4& q) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(as2(q.x), as2(q.y)), __hmax2(as2(q.z), as2(q.w)));
+    return fmaxf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ float one(const uint8_t* p) {
     return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16);
@@ -204,10 +251,16 @@ struct Vec<DT_BF16> {
 template <>
 struct Vec<DT_F32> {
   static constexpr int N = 4, ES = 4;
-  static __device__ __forceinline__ float unpack(const uint4& q, float (&x)[4]) {
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[4]) {
     x[0] = __uint_as_float(q.x); x[1] = __uint_as_float(q.y);
     x[2] = __uint_as_float(q.z); x[3] = __uint_as_float(q.w);
-    return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  }
+  static __device__ __forceinline__ uint4 unmask(const uint4& q) {
+    return make_uint4(__float_as_uint(max_nan(__uint_as_float(q.x), -3.0e38f)), __float_as_uint(max_nan(__uint_as_float(q.y), -3.0e38f)),
+                      __float_as_uint(max_nan(__uint_as_float(q.z), -3.0e38f)), __float_as_uint(max_nan(__uint_as_float(q.w), -3.0e38f)));
+  }
+  static __device__ __forceinline__ float max_of(const uint4& q) {
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
   }
   static __device__ __forceinline__ float one(const uint8_t* p) { return *reinterpret_cast<const float*>(p); }
 };
@@ -220,12 +273,42 @@ __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
   return q;
 }
 
+constexpr int CAP = 512;                 // candidate keys
+static_assert(WARPS * 32 <= CAP, "the warps' lists are ranked in the same array");
+
 struct Shared {
   Acc warp_acc[WARPS];
-  u64 warp_keys[WARPS][32];
   Acc cta_acc[MAX_CLUSTER];              // written by the cluster's CTAs into the first one's copy
-  u64 cta_keys[MAX_CLUSTER][32];
 };
+struct alignas(16) TopShared {
+  u64 cand[CAP];
+  u64 best[32];                          // ranked, descending
+  u64 cta_keys[MAX_CLUSTER * 32];        // as cta_acc
+  float warp_bound[WARPS];
+  int count;
+};
+
+// the best 32 of cand[0 .. n) in order of rank, into best[] (0 where there are fewer); all threads call it
+__device__ __forceinline__ void rank_keys(const u64* cand, int n, u64* best) {
+  if (threadIdx.x < 32) best[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const u64 mine = cand[i];
+    if (mine == 0) continue;
+    int above = 0;
+    int j = 0;
+    for (; j + 8 <= n; j += 8) {
+#pragma unroll
+      for (int u = 0; u < 8; u += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(cand + j + u);
+        above += (q.x > mine) + (q.y > mine);
+      }
+    }
+    for (; j < n; ++j) above += cand[j] > mine;
+    if (above < 32) best[above] = mine;
+  }
+  __syncthreads();
+}
 
 // what the joined row comes to; `keys` of warp 0's lanes
 __device__ __forceinline__ void write_row(const Params& p, long long row, const Acc& a, float zt, bool found, bool top,
@@ -239,16 +322,19 @@ __device__ __forceinline__ void write_row(const Params& p, long long row, const 
     if (p.lse) p.lse[row] = a.m + log_s;
   }
   if (top && lane < p.top_k) {
-    p.top_ids[row * p.top_k + lane] = static_cast<long long>(key_index(list));
-    p.top_logprobs[row * p.top_k + lane] = (key_value(list) * p.inv_t - a.m) - log_s;
+    // fewer than k comparable logits (NaN): any valid column
+    p.top_ids[row * p.top_k + lane] = list != 0 ? static_cast<long long>(key_index(list)) : lane;
+    p.top_logprobs[row * p.top_k + lane] = ((list != 0 ? key_value(list) : NAN) * p.inv_t - a.m) - log_s;
   }
 }
 
 template <int DT, bool TOP>
-__global__ void __launch_bounds__(THREADS) logprobs_kernel(const Params p, const int cs) {
+__global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(const Params p, const int cs) {
   using V = Vec<DT>;
   constexpr int N = V::N, ES = V::ES;
   __shared__ Shared sh;
+  __shared__ typename std::conditional<TOP, TopShared, char>::type top_raw;
+  TopShared& top = reinterpret_cast<TopShared&>(top_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long row = blockIdx.x / cs;
   const int rank = blockIdx.x % cs;
@@ -257,117 +343,209 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const Params p, const
 
   // columns: `head` up to the first 16-byte boundary, nv whole vectors shared out over the cluster, a tail
   const int mis = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / ES;
-  const long long head = mis < p.vocab ? mis : p.vocab;
-  const long long nv = (p.vocab - head) / N;
-  const long long tail0 = head + nv * N;
-  const uint8_t* vbase = base + head * ES;
+  const int vocab = static_cast<int>(p.vocab);
+  const int head = mis < vocab ? mis : vocab;
+  const int nv = (vocab - head) / N;
+  const int tail0 = head + nv * N;
+  const uint8_t* vbase = base + static_cast<long long>(head) * ES;
   // whole warps of vectors per CTA
-  const long long per = ((nv + cs - 1) / cs + 31) / 32 * 32;
-  const long long v_begin = rank * per < nv ? rank * per : nv;
-  const long long v_end = v_begin + per < nv ? v_begin + per : nv;
+  const int per = ((nv + cs - 1) / cs + 31) / 32 * 32;
+  const int v_begin = min(rank * per, nv), v_end = min(v_begin + per, nv);
 
   const float c = p.inv_t * LOG2E;
   const float lazy = LAZY_LOG / p.inv_t;
   Run r;
   r.m = -INFINITY;
   r.thr = -INFINITY;
+  r.nm = 0.0f;
   r.s = r.t = make_float2(0.0f, 0.0f);
-  u64 list = 0, floor_key = 0;
-  float floor_val = -INFINITY;           // the k-th best value so far (-inf: the list is not full)
 
-  auto offer = [&](const float* x, int n, float vmax, long long first, bool live) {
-    if constexpr (TOP) {
-      if (__any_sync(0xffffffffu, live && vmax >= floor_val)) {
-        for (int i = 0; i < n; ++i) {
-          const u64 key = live ? make_key(x[i], static_cast<uint32_t>(p.vocab_start + first + i)) : 0;
-          warp_insert(list, floor_key, key, p.top_k, lane);
-        }
-        floor_val = floor_key != 0 ? key_value(floor_key) : -INFINITY;
-      }
-    }
-  };
+  // the given token's logit, asked for now and used at the end
+  const long long t = p.targets ? p.targets[row] : p.ignore_index;
+  const long long tl = t - p.vocab_start;
+  const bool found = rank == 0 && t != p.ignore_index && t >= 0 && t < p.vocab_total && tl >= 0 && tl < p.vocab;
+  const float zt = found ? V::one(base + tl * ES) * p.inv_t : 0.0f;
 
   constexpr int U = 4;
-  long long v = v_begin + warp * 32;
-  for (; v + (U - 1) * THREADS + 32 <= v_end; v += U * THREADS) {
-    uint4 q[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = load_stream(vbase + (v + u * THREADS + lane) * 16);
+  float bound = -INFINITY;               // nothing below it can be among the best k
+  if constexpr (TOP) {
+    if (threadIdx.x == 0) top.count = 0;
+    __syncthreads();
+  }
+  auto push = [&](float x, int col) {
+    const int at = atomicAdd(&top.count, 1);
+    if (at < CAP) top.cand[at] = make_key(x, static_cast<uint32_t>(p.vocab_start) + col);
+  };
+  // candidates -> the best 32 of them and a new bound; false if there were too many to keep
+  auto rank_down = [&]() {
+    __syncthreads();
+    const int n = top.count;
+    if (n > CAP) return false;
+    rank_keys(top.cand, n, top.best);
+    if (threadIdx.x < 32) top.cand[threadIdx.x] = top.best[threadIdx.x];
+    if (threadIdx.x == 0) top.count = 32;
+    const u64 kth = top.best[p.top_k - 1];
+    if (kth != 0) bound = key_value(kth);
+    __syncthreads();
+    return true;
+  };
+  bool kept = true;                      // every candidate is in top.cand
+
+  // vectors past the end are all masked
+  auto load = [&](int v0, uint4 (&q)[U]) {
+    const uint32_t lo = DT == DT_BF16 ? 0xff80ff80u : 0xff800000u;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float x[N];
-      const float vmax = V::unpack(q[u], x);
-      accumulate<N>(r, x, vmax, lazy, c);
-      offer(x, N, vmax, head + (v + u * THREADS + lane) * N, true);
+      const int v = v0 + u * THREADS + threadIdx.x;
+      q[u] = make_uint4(lo, lo, lo, lo);
+      if (v < v_end) q[u] = load_stream(vbase + static_cast<long long>(v) * 16);
     }
-  }
-  for (; v < v_end; v += THREADS) {
-    const bool live = v + lane < v_end;
-    float x[N];
-    float vmax = -INFINITY;
-    if (live) {
-      vmax = V::unpack(load_stream(vbase + (v + lane) * 16), x);
-      accumulate<N>(r, x, vmax, lazy, c);
+  };
+  uint4 q[U], ahead[U];
+  load(v_begin, ahead);
+  for (int v0 = v_begin, batch = 1, next_rank = 1; v0 < v_end; v0 += U * THREADS, ++batch) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = ahead[u];
+    if (v0 + U * THREADS < v_end) load(v0 + U * THREADS, ahead);
+    float mx = V::max_of(q[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) mx = fmaxf(mx, V::max_of(q[u]));
+    if (mx > r.thr) rebase(r, mx, lazy, c);
+    float2 t = make_float2(0.0f, 0.0f);
+    const Run before = r;
+    // (a maximum as low as what stands for a masked logit: take them as they are)
+    if (r.m > -1.0e38f) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[N];
+        V::unpack(V::unmask(q[u]), x);
+        accumulate<N>(r, t, x, c);
+      }
     }
-    offer(x, N, vmax, head + (v + lane) * N, live);
+    const float tt = t.x + t.y;
+    if (r.m > -1.0e38f && tt == tt) {
+      r.t = fadd2(r.t, t);
+    } else {
+      r = before;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[N];
+        V::unpack(q[u], x);
+        accumulate_raw<N>(r, x, c);
+      }
+    }
+    if constexpr (TOP) {
+      if (v0 == v_begin) {
+        // the first bound, from the threads' maxima of this batch
+        const int full = min(WARPS, (v_end - v_begin) / 32);         // warps whose first vectors are all live
+        if (full > 0 && warp < full) {
+          const int need = (p.top_k + full - 1) / full;
+          uint32_t key = static_cast<uint32_t>(make_key(mx, 0) >> 32);
+          uint32_t best = 0;
+          for (int i = 0; i < need; ++i) {
+            best = __reduce_max_sync(0xffffffffu, key);
+            const int first = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
+            if (lane == first) key = 0;
+          }
+          if (lane == 0) top.warp_bound[warp] = best == 0 ? -INFINITY : key_value(static_cast<u64>(best) << 32);
+        }
+        __syncthreads();
+        if (full > 0) {
+          bound = top.warp_bound[0];
+          for (int w = 1; w < full; ++w) bound = fminf(bound, top.warp_bound[w]);
+        }
+      }
+      if (kept && mx >= bound) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int v = v0 + u * THREADS + threadIdx.x;
+          if (v < v_end && V::max_of(q[u]) >= bound) {
+            float x[N];
+            V::unpack(q[u], x);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              if (x[i] >= bound) push(x[i], head + v * N + i);
+          }
+        }
+      }
+      if (batch == next_rank && v0 + U * THREADS < v_end) {
+        next_rank *= 4;
+        kept = kept && rank_down();
+      }
+    }
   }
   // at most N - 1 single columns at either end: warp 0 of the first CTA, one per lane
   if (rank == 0 && warp == 0) {
-    const int n_tail = static_cast<int>(p.vocab - tail0);
-    const int n_one = static_cast<int>(head) + n_tail;
-    const bool live = lane < n_one;
-    const long long col = lane < head ? lane : tail0 + (lane - head);
-    float x[2] = {-INFINITY, -INFINITY};
-    if (live) {
-      x[0] = V::one(base + col * ES);
-      accumulate<2>(r, x, x[0], lazy, c);
+    const int n_one = head + vocab - tail0;
+    const int col = lane < head ? lane : tail0 + (lane - head);
+    if (lane < n_one) {
+      const float x[1] = {V::one(base + static_cast<long long>(col) * ES)};
+      if (x[0] > r.thr) rebase(r, x[0], lazy, c);
+      accumulate_raw<1>(r, x, c);
+      if (TOP && x[0] >= bound) push(x[0], col);
     }
-    offer(x, 1, x[0], col, live);
   }
 
   // raw units -> units of z
   Acc a{r.m == -INFINITY ? r.m : r.m * p.inv_t, r.s.x + r.s.y, (r.t.x + r.t.y) * p.inv_t};
   a = warp_join(a);
   if (lane == 0) sh.warp_acc[warp] = a;
-  if constexpr (TOP) sh.warp_keys[warp][lane] = list;
   __syncthreads();
-  if (warp == 0) {
-    a = warp_join(lane < WARPS ? sh.warp_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
-    if constexpr (TOP) {
-      for (int w = 1; w < WARPS; ++w) list = warp_merge(list, sh.warp_keys[w][lane], lane);
+  if (warp == 0) a = warp_join(lane < WARPS ? sh.warp_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
+  if constexpr (TOP) {
+    int n = top.count;
+    __syncthreads();
+    if (n > CAP) {
+      // once more, each warp for itself
+      u64 list = 0, floor_key = 0;
+      for (int v0 = v_begin + warp * 32; v0 < v_end; v0 += THREADS) {
+        const int v = v0 + lane;
+        float x[N];
+        if (v < v_end) V::unpack(load_stream(vbase + static_cast<long long>(v) * 16), x);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          warp_offer(list, floor_key, v < v_end ? make_key(x[i], static_cast<uint32_t>(p.vocab_start) + head + v * N + i) : 0, p.top_k, lane);
+      }
+      if (rank == 0 && warp == 0) {
+        const int col = lane < head ? lane : tail0 + (lane - head);
+        warp_offer(list, floor_key,
+                   lane < head + vocab - tail0 ? make_key(V::one(base + static_cast<long long>(col) * ES), static_cast<uint32_t>(p.vocab_start) + col) : 0,
+                   p.top_k, lane);
+      }
+      top.cand[warp * 32 + lane] = list;
+      n = WARPS * 32;
+      __syncthreads();
     }
+    rank_keys(top.cand, n, top.best);
   }
   if (cs > 1) {
+    __syncwarp();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");       // the first CTA has started
     cg::cluster_group cluster = cg::this_cluster();
     if (warp == 0) {
       Shared* first = cluster.map_shared_rank(&sh, 0);
       if (lane == 0) first->cta_acc[rank] = a;
-      if constexpr (TOP) first->cta_keys[rank][lane] = list;
-    }
-    cluster.sync();
-    if (rank == 0 && warp == 0) {
-      a = warp_join(lane < cs ? sh.cta_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
       if constexpr (TOP) {
-        for (int w = 1; w < cs; ++w) list = warp_merge(list, sh.cta_keys[w][lane], lane);
+        if (lane < p.top_k) cluster.map_shared_rank(&top, 0)->cta_keys[rank * p.top_k + lane] = top.best[lane];
       }
     }
+    __syncwarp();
+    cluster.sync();
+    if (rank != 0) return;
+    if (warp == 0) a = warp_join(lane < cs ? sh.cta_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
+    if constexpr (TOP) rank_keys(top.cta_keys, cs * p.top_k, top.best);
   }
-  if (rank != 0 || warp != 0) return;
+  if (warp != 0) return;
 
-  // the given token: one load by every lane of the warp
-  const long long t = p.targets ? p.targets[row] : p.ignore_index;
-  const long long tl = t - p.vocab_start;
-  const bool found = t != p.ignore_index && t >= 0 && t < p.vocab_total && tl >= 0 && tl < p.vocab;
-  const float zt = found ? V::one(base + tl * ES) * p.inv_t : 0.0f;
+  const u64 key = TOP ? top.best[lane] : 0;
   if (p.stats != nullptr) {
     if (lane == 0) {
       float* s = p.stats + row * 5;
       s[0] = a.m; s[1] = a.s; s[2] = a.t; s[3] = zt; s[4] = found ? 1.0f : 0.0f;
     }
-    if (TOP && lane < p.top_k) p.keys[row * p.top_k + lane] = list;
+    if (TOP && lane < p.top_k) p.keys[row * p.top_k + lane] = key;
   } else {
-    write_row(p, row, a, zt, found, TOP, list, lane);
+    write_row(p, row, a, zt, found, TOP, key, lane);
   }
 }
 
@@ -422,15 +600,19 @@ __device__ __forceinline__ void store_one(uint8_t* p, float x) {
   else *reinterpret_cast<float*>(p) = x;
 }
 
-constexpr int BACK_THREADS = 256;
+// small CTAs with all of their loads in flight at once: 4095 x 151936 bf16 with an entropy gradient takes 367 us with 128
+// threads of eight vectors each, 402 with four, 415 / 414 with 256 threads of four / eight, 472 with 512 of two
+constexpr int BACK_THREADS = 128;
+constexpr int BACK_VECS = 8;
 
 // grid: (column chunks, rows folded over y and z)
 template <int DT, bool ENT>
 __global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const BackParams p, long long rows, int vec_per_cta) {
   using V = Vec<DT>;
   constexpr int N = V::N, ES = V::ES;
-  const long long row = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
-  if (row >= rows) return;
+  // the last rows first: they are what the forward pass has left in the L2
+  const long long row = rows - 1 - (blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y);
+  if (row < 0) return;
   const uint8_t* in = p.logits + row * p.ld * ES;
   uint8_t* out = p.grad + row * p.ld_grad * ES;
   const long long t = p.targets ? p.targets[row] : p.ignore_index;
@@ -458,7 +640,7 @@ __global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const B
   const long long nv = (p.vocab - head) / N;
   const long long v_begin = static_cast<long long>(blockIdx.x) * vec_per_cta;
   const long long v_end = v_begin + vec_per_cta < nv ? v_begin + vec_per_cta : nv;
-  constexpr int U = 4;
+  constexpr int U = BACK_VECS;
   for (long long v = v_begin + threadIdx.x; v < v_end; v += U * BACK_THREADS) {
     uint4 q[U];
 #pragma unroll
@@ -572,12 +754,13 @@ extern "C" int forge_logprobs_forward(const ForgeLogprobsArgs* args, void* cuda_
   const DeviceInfo* di = current_device_info();
   if (di == nullptr) return FORGE_ERR_CUDA;
   if (di->cc_major != 10) return fail(FORGE_ERR_DEVICE, "device %d is sm_%d%d, not sm_100", di->device, di->cc_major, di->cc_minor);
-  // A row is cut over as many CTAs as keep the GPU's CTA slots (four of 512 threads per SM) filled, while each
-  // still has a batch of vectors per thread to load.
-  const long long slots = 4ll * di->sm_count;
+  // A row is cut over a cluster while two CTAs per SM hold all of them and each still has two vectors per thread
+  // to load: 64 rows of 128256 bf16 logits take 14.6 / 9.7 / 7.7 / 10.2 us over 1 / 2 / 4 / 8 CTAs a row, 4096 fp32
+  // logits 4.7 / 5.9 us over 1 / 2.  The first CTA ranks the others' k keys each: with k = 20, 8 CTAs a row beat 16
+  // (14.6 against 18.5 us for 16 rows).
   const long long vecs = a.vocab * es / 16;
   int cs = 1;
-  while (cs < loss::MAX_CLUSTER && a.rows * cs * 2 <= slots && vecs > static_cast<long long>(cs) * loss::THREADS) cs *= 2;
+  while (cs < loss::MAX_CLUSTER && a.rows * cs * 2 <= 2ll * di->sm_count && vecs > 4ll * cs * loss::THREADS && cs * 2 * a.top_k <= 192) cs *= 2;
   const loss::Params p = loss::make_params(a);
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   if (a.dtype == FORGE_DT_BF16)
@@ -627,8 +810,7 @@ extern "C" int forge_logprobs_backward(const ForgeLogprobsArgs* args, const floa
   p.vocab = a.vocab; p.ld = a.ld; p.ld_grad = ld_grad; p.ignore_index = a.ignore_index;
   p.vocab_start = a.vocab_start; p.vocab_total = a.vocab_total;
   p.inv_t = static_cast<float>(1.0 / a.temperature);
-  // 16 KB of logits per CTA (four 16-byte loads per thread)
-  const int vec_per_cta = loss::BACK_THREADS * 4;
+  const int vec_per_cta = loss::BACK_THREADS * loss::BACK_VECS;
   const long long vecs = a.vocab * es / 16;
   const long long chunks = std::max<long long>(1, (vecs + vec_per_cta - 1) / vec_per_cta);
   const unsigned gy = static_cast<unsigned>(std::min<int64_t>(a.rows, 32768));

@@ -138,6 +138,23 @@ def test_rows_without_a_distribution():
     assert dx[~bad].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(3, 70001), (400, 70001)])
+def test_alternatives_of_hard_rows(dtype, rows, vocab):
+    """Rows in which nearly every element passes for a candidate, for one CTA per row and for many."""
+    x, t = make(rows, vocab, dtype, seed=21)
+    x[0] = 1.0                                                              # all tie
+    x[1] = torch.linspace(-9, 9, vocab, device=DEV).to(dtype)               # ascending, with ties in bf16
+    x[2] = -math.inf
+    x[2, vocab - 3:] = torch.tensor([1.0, 2.0, 2.0], device=DEV).to(dtype)  # three columns left
+    for k in (1, 5, 32):
+        check(x, t, top_k=k, grads=False)
+    x[0] = math.nan
+    out = token_logprobs(x, t, top_k=32)
+    assert out.logprobs[0].isnan() and out.top_logprobs[0].isnan().all()
+    assert (out.top_ids >= 0).all() and (out.top_ids < vocab).all()
+
+
 def test_targets_outside_the_vocabulary():
     x, t = make(4, 515, torch.bfloat16, seed=11)
     x = x.requires_grad_(True)
