@@ -206,6 +206,7 @@ _SIGNATURES = {
     "forge_multi_norm": (ctypes.c_int, [ctypes.POINTER(ForgeNormItem), ctypes.c_int32, ctypes.c_double, ctypes.c_void_p,
                                         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "forge_fp8_quantize": (ctypes.c_int, [ctypes.POINTER(ForgeFp8QuantizeArgs), ctypes.c_void_p]),
+    "forge_fp8_linear": (ctypes.c_int, [ctypes.POINTER(ForgeFp8QuantizeArgs), ctypes.POINTER(ForgeFp8ProductArgs), ctypes.c_void_p]),
     "forge_fp8_product": (ctypes.c_int, [ctypes.POINTER(ForgeFp8ProductArgs), ctypes.c_void_p]),
     "forge_state_bytes": (
         ctypes.c_int,

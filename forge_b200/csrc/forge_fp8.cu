@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "forge_host.h"
 #include "forge_ptx.cuh"
@@ -76,10 +77,15 @@ struct QuantParams {
   long long rows, cols, ld_x, ld_q, ld_qt;
 };
 
+// programmatic dependent launch: the kernel that follows may start / wait for the one before and see what it wrote
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // 1 x 128 blocks: sixteen lanes of eight columns each; a warp takes two neighbouring blocks of a row
 template <int DT>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p) {
   constexpr int ES = DT == DT_BF16 ? 2 : 4;
+  allow_next();
   const int lane = threadIdx.x & 31;
   const long long cb = (p.cols + 127) / 128, pairs = (cb + 1) / 2;
   const long long unit = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -203,14 +209,16 @@ struct Params {
   int tiles_m;
   int split;
   int wide;                                         // rows of y are 16-byte aligned
+  int early;                                        // launched while the kernel that writes X's codes may still run
   int* status;
 };
 
-enum : int { ERR_OP_EMPTY = 221, ERR_OP_FULL = 222, ERR_ACC_EMPTY = 223, ERR_ACC_FULL = 224 };
+enum : int { ERR_OP_EMPTY = 221, ERR_OP_FULL = 222, ERR_ACC_EMPTY = 223, ERR_ACC_FULL = 224, ERR_SC_EMPTY = 225, ERR_SC_FULL = 226 };
+constexpr int SC_SLOTS = 8;                         // K blocks whose scales are in shared memory
 constexpr int BK = 128;                             // bytes = elements
 constexpr int A_BYTES = 128 * BK;
 constexpr int ACC_BUFS = 4;
-constexpr int THREADS = 256;
+constexpr int THREADS = 384;                        // producer, MMA, two idle warps; eight epilogue warps
 
 template <int NT>
 struct Cfg {
@@ -222,6 +230,14 @@ struct Cfg {
   static constexpr int TMEM_COLS = ACC_BUFS * NT;
   static constexpr int MIN_CTAS = NT == 128 ? 1 : 2;
 };
+
+// 32 lanes x 8 consecutive columns
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
 
 // instruction descriptor of kind::f8f6f4, e4m3 x e4m3 -> f32, both operands K-major
 __host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) {
@@ -251,16 +267,50 @@ struct Ctrl {
   uint64_t empty[8];
   uint64_t acc_full[ACC_BUFS];
   uint64_t acc_empty[ACC_BUFS];
+  uint64_t sc_full[SC_SLOTS];
+  uint64_t sc_empty[SC_SLOTS];
   uint32_t tmem_base;
   int abort_word;
 };
+
+// The scales' products sx sw of one K block after the other, formed by two warps (64 threads) and handed to the
+// epilogue through slots of W floats: loaded where they are used, they cost the epilogue a memory latency per K block.
+// Four blocks are asked for at a time.  value(i, kb): what thread-slot i holds for block kb.
+template <int W, typename F>
+__device__ __forceinline__ bool feed_scales(float (*sc)[W], uint64_t* full, uint64_t* empty, int& it, int kb0, int kb1, volatile int* abort_word,
+                                            F&& value) {
+  const int t = threadIdx.x - 64;
+  constexpr int PER = (W + 63) / 64;
+  for (int kb = kb0; kb < kb1; kb += 4) {
+    float v[4][PER];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[u][i] = kb + u < kb1 && t + 64 * i < W ? value(t + 64 * i, kb + u) : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (kb + u >= kb1) break;
+      const int slot = it % SC_SLOTS;
+      bool ok = mbar_wait(&empty[slot], ((it / SC_SLOTS) & 1) ^ 1, abort_word, ERR_SC_EMPTY);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return false;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (t + 64 * i < W) sc[slot][t + 64 * i] = v[u][i];
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&full[slot]);
+      ++it;
+    }
+  }
+  return true;
+}
 
 template <int NT>
 __global__ void __launch_bounds__(THREADS, Cfg<NT>::MIN_CTAS)
 fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params p) {
   using C = Cfg<NT>;
   __shared__ Ctrl ctrl;
-  __shared__ __align__(16) float sc[2][NT];
+  __shared__ __align__(16) float sc[SC_SLOTS][NT];
   extern __shared__ uint8_t smem_raw[];
   uint8_t* data = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -274,7 +324,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; ++i) { mbar_init(&ctrl.full[i], 1); mbar_init(&ctrl.empty[i], 1); }
-    for (int i = 0; i < ACC_BUFS; ++i) { mbar_init(&ctrl.acc_full[i], 1); mbar_init(&ctrl.acc_empty[i], 4); }
+    for (int i = 0; i < ACC_BUFS; ++i) { mbar_init(&ctrl.acc_full[i], 1); mbar_init(&ctrl.acc_empty[i], 8); }
+    for (int i = 0; i < SC_SLOTS; ++i) { mbar_init(&ctrl.sc_full[i], 2); mbar_init(&ctrl.sc_empty[i], 8); }
     ctrl.abort_word = 0;
     mbar_fence_init();
   }
@@ -295,14 +346,23 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     if (lane == 0) {
       const uint64_t pol_w = p.tiles_m > 1 ? policy_evict_normal() : policy_evict_first();
       const uint64_t pol_x = policy_evict_last();
+      // (early: the weight's first stages are asked for before the tokens' codes are known to be there)
+      auto second_operand = [&]() {
+        wait_for_previous();
+        for (int i = 0; i < min(C::STAGES, kb1 - kb0); ++i)
+          tma_load_2d(data + i * C::STAGE + A_BYTES, &tm_x, &ctrl.full[i], (kb0 + i) * BK, m0, pol_x);
+      };
       for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
         const int s = it % C::STAGES;
+        if (p.early && it == C::STAGES) second_operand();
         if (!mbar_wait(&ctrl.empty[s], ((it / C::STAGES) & 1) ^ 1, abort_word, ERR_OP_EMPTY)) break;
         uint8_t* a = data + s * C::STAGE;
         mbar_expect_tx(&ctrl.full[s], C::STAGE);
         tma_load_2d(a, &tm_w, &ctrl.full[s], kb * BK, n0, pol_w);
+        if (p.early && it < C::STAGES) continue;
         tma_load_2d(a + A_BYTES, &tm_x, &ctrl.full[s], kb * BK, m0, pol_x);
       }
+      if (p.early && kb1 - kb0 <= C::STAGES) second_operand();
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -321,38 +381,38 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
         umma_commit(&ctrl.acc_full[b]);
       }
     }
-  } else if (warp >= 4) {
-    const int quarter = warp & 3, e = threadIdx.x - 128;
-    float acc[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
-    // this thread fetches the scale of token m0 + e for the coming blocks
-    const bool has = e < NT && m0 + e < p.M;
-    const float* sxp = p.sx + static_cast<long long>(m0 + (has ? e : 0)) * p.sx_row;
+  } else if (warp < 4) {
+    if (p.early) wait_for_previous();
     const float* swp = p.sw + static_cast<long long>(n0 / 128) * p.sw_row;
-    auto fetch = [&](int kb) { return has && kb < kb1 ? sxp[kb * p.sx_col] * swp[kb * p.sw_col] : 0.0f; };
-    float s_next = fetch(kb0), s_next2 = fetch(kb0 + 1);
-    bool ok = true;
-    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-      const int b = it % ACC_BUFS;
-      if (e < NT) sc[it & 1][e] = s_next;
-      s_next = s_next2;
-      s_next2 = fetch(kb + 2);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      ok = mbar_wait(&ctrl.acc_full[b], (it / ACC_BUFS) & 1, abort_word, ERR_ACC_FULL) && ok;
-      tc_fence_after();
-      __syncwarp();
-      constexpr int STEP = NT < 32 ? 16 : 32;
+    int it = 0;
+    feed_scales<NT>(sc, ctrl.sc_full, ctrl.sc_empty, it, kb0, kb1, abort_word, [&](int i, int kb) {
+      return m0 + i < p.M ? p.sx[static_cast<long long>(m0 + i) * p.sx_row + kb * p.sx_col] * swp[kb * p.sw_col] : 0.0f;
+    });
+  } else {
+    // two warpgroups, each with half of the tokens
+    constexpr int NC = NT / 2;
+    const int quarter = warp & 3, c0 = ((warp - 4) >> 2) * NC;
+    float acc[NC];
 #pragma unroll
-      for (int c = 0; c < NT; c += STEP) {
+    for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
+    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+      const int b = it % ACC_BUFS, slot = it % SC_SLOTS;
+      bool ok = mbar_wait(&ctrl.sc_full[slot], (it / SC_SLOTS) & 1, abort_word, ERR_SC_FULL);
+      ok = mbar_wait(&ctrl.acc_full[b], (it / ACC_BUFS) & 1, abort_word, ERR_ACC_FULL) && ok;
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      constexpr int STEP = NC < 32 ? NC : 32;
+#pragma unroll
+      for (int c = 0; c < NC; c += STEP) {
         uint32_t r[STEP];
-        const uint32_t ta = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + b * NT + c;
-        if constexpr (STEP == 16) tmem_ld_32x16(ta, r);
+        const uint32_t ta = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + b * NT + c0 + c;
+        if constexpr (STEP == 8) tmem_ld_32x8(ta, r);
+        else if constexpr (STEP == 16) tmem_ld_32x16(ta, r);
         else tmem_ld_32x32(ta, r);
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < STEP; j += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(&sc[it & 1][c + j]);
+          const float4 s4 = *reinterpret_cast<const float4*>(&sc[slot][c0 + c + j]);
           const float2 lo = ffma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(s4.x, s4.y),
                                   make_float2(acc[c + j], acc[c + j + 1]));
           const float2 hi = ffma2(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), make_float2(s4.z, s4.w),
@@ -362,14 +422,17 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl.acc_empty[b]);
+      if (lane == 0) {
+        mbar_arrive(&ctrl.acc_empty[b]);
+        mbar_arrive(&ctrl.sc_empty[slot]);
+      }
     }
     // Every product has completed (the last accumulator was signalled after all of them), so the operand
     // stages are free: the part goes there as [token][weight row].
     float* part = reinterpret_cast<float*>(data);
     const int r = quarter * 32 + lane;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) part[j * 128 + r] = acc[j];
+    for (int j = 0; j < NC; ++j) part[(c0 + j) * 128 + r] = acc[j];
   }
   __syncwarp();
   tc_fence_before();
@@ -418,26 +481,295 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   }
 }
 
-template <int NT>
-static int launch_product(const CUtensorMap& tw, const CUtensorMap& tx, const Params& p, int ctas, cudaStream_t stream) {
-  auto* fn = fp8_product_kernel<NT>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NT>::SMEM);
+// sets a kernel's shared-memory limit once per device
+template <typename F>
+static int allow_smem(F* fn, int bytes, std::atomic<uint64_t>& done, int device) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return FORGE_OK;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "fp8 product: shared memory attribute: %s", cudaGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return FORGE_OK;
+}
+
+// a launch of clusters; `early`: it may begin before the kernel in front of it in the stream has ended
+struct Launch {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = Cfg<NT>::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, fn, tw, tx, p);
+  cudaLaunchAttribute attr[2];
+  Launch(int ctas, int threads, int smem, int cluster, bool early, cudaStream_t stream) {
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = early ? 2 : 1;
+  }
+};
+
+template <int NT>
+static int launch_product(const CUtensorMap& tw, const CUtensorMap& tx, const Params& p, int ctas, int device, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  auto* fn = fp8_product_kernel<NT>;
+  const int rc = allow_smem(fn, Cfg<NT>::SMEM, done, device);
+  if (rc != FORGE_OK) return rc;
+  Launch l(ctas, THREADS, Cfg<NT>::SMEM, p.split, p.early, stream);
+  cudaError_t e = cudaLaunchKernelEx(&l.cfg, fn, tw, tx, p);
   if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "fp8 product launch: %s", cudaGetErrorString(e));
   return FORGE_OK;
 }
+
+// ---------------------------------------------------------------------------------------------
+// product, a pair of CTAs per tile of 256 tokens x 256 weight rows
+// ---------------------------------------------------------------------------------------------
+// For many tokens.  The pair's MMA (cta_group::2) reads each CTA's 128 tokens and half of the tile's weight rows from that
+// CTA's shared memory, so a CTA stages 32 KB per K block for 128 x 256 x 128 products, half of what single CTAs of
+// 128 x 128 stage per product.  Tokens are the accumulator's
+// rows: a thread's scale is then one number per K block, sx[its token, kb] sw[its 128 weight rows, kb].  Every K block
+// goes to an accumulator of its own (two of 256 columns); eight warps add it, scaled, to 128 fp32 registers each thread
+// while the tensor cores work on the next one.
+//
+// 4096 x 14336 x 4096: 228 us, 2.1 PFLOP/s.  The MMAs alone, on operands that stay in place, take 156 us; with the copies of
+// the operands 194 (four or five stages alike: the copies and the MMAs' operand reads share the shared memory's
+// bandwidth); the rest is the hand-over of an accumulator per K block.  Four column groups of 64 instead of two of 128
+// (less work per warp, but 112 registers are too few): 245 to 270 us; 32 columns per fetch instead of 16: 233 us.
+namespace pair {
+constexpr int STAGES = 5;
+constexpr int STAGE = 2 * A_BYTES;                    // 128 tokens and 128 weight rows
+constexpr int OUT_BYTES = 128 * 256 * 2;
+constexpr int SMEM = 1024 + STAGES * STAGE + OUT_BYTES;
+constexpr int GROUPS = 2;                             // epilogue warpgroups, each with 256 / GROUPS columns
+constexpr int COLS = 256 / GROUPS;
+constexpr int THREADS = 128 + GROUPS * 128;           // producer, MMA, two idle warps; the epilogue
+constexpr int TMEM_COLS = 512;
+
+struct Ctrl {
+  uint64_t full[STAGES];
+  uint64_t empty[STAGES];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  int abort_word;
+};
+
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+constexpr int STEP = 16;                              // columns fetched from tensor memory at a time
+// acc += s * STEP columns of the accumulator
+__device__ __forceinline__ void add_scaled(float2 (&acc)[COLS / 2], int at, const uint32_t (&r)[STEP], float s) {
+  const float2 s2 = make_float2(s, s);
+#pragma unroll
+  for (int j = 0; j < STEP / 2; ++j)
+    acc[at + j] = ffma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[at + j]);
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                const __grid_constant__ CUtensorMap tm_out, const Params p) {
+  __shared__ Ctrl ctrl;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* data = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* out_buf = data + STAGES * STAGE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_word = &ctrl.abort_word;
+  const uint32_t cta_rank = cluster_ctarank();
+  const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(gridDim.x) / 2;
+  const int num_tiles = p.tiles_m * ((p.N + 255) / 256);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) { mbar_init(&ctrl.full[i], 1); mbar_init(&ctrl.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&ctrl.acc_full[i], 1); mbar_init(&ctrl.acc_empty[i], 8 * GROUPS); }
+    ctrl.abort_word = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&ctrl.tmem_base, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
+    if (p.wide) prefetch_tmap(&tm_out);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();          // the peer's barriers exist before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem_base = ctrl.tmem_base;
+
+  if (warp < 4) {
+    setmaxnreg_dec<40>();
+    if (warp == 0 && lane == 0) {
+      const uint64_t pol = policy_evict_normal();
+      if (p.early) wait_for_previous();
+      int it = 0;
+      for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
+        const int m0 = (tile % p.tiles_m) * 256 + static_cast<int>(cta_rank) * 128;
+        const int n0 = (tile / p.tiles_m) * 256 + static_cast<int>(cta_rank) * 128;
+        for (int kb = 0; kb < p.KB; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&ctrl.empty[s], ((it / STAGES) & 1) ^ 1, abort_word, ERR_OP_EMPTY)) goto done;
+          uint8_t* a = data + s * STAGE;
+          // both CTAs' copies count on the leader's barrier, which expects the bytes of both
+          const uint32_t full_leader = map_to_cta(smem_u32(&ctrl.full[s]), 0);
+          if (cta_rank == 0) mbar_expect_tx(&ctrl.full[s], 2 * STAGE);
+          tma_load_2d_pair(a, &tm_x, full_leader, kb * BK, m0, pol);
+          tma_load_2d_pair(a + A_BYTES, &tm_w, full_leader, kb * BK, n0, pol);
+        }
+      }
+    } else if (warp == 1 && lane == 0 && cta_rank == 0) {
+      constexpr uint32_t idesc = make_idesc_e4m3(256, 256);
+      int it = 0;
+      for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
+        for (int kb = 0; kb < p.KB; ++kb, ++it) {
+          const int s = it % STAGES, b = it & 1;
+          if (!mbar_wait(&ctrl.acc_empty[b], ((it >> 1) & 1) ^ 1, abort_word, ERR_ACC_EMPTY)) goto done;
+          if (!mbar_wait(&ctrl.full[s], (it / STAGES) & 1, abort_word, ERR_OP_FULL)) goto done;
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(data + s * STAGE), b_addr = a_addr + A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            umma_f8_pair(tmem_base + b * 256, make_smem_desc_sw128(a_addr + k * 32, 16, 1024),
+                         make_smem_desc_sw128(b_addr + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
+          umma_commit_pair(&ctrl.empty[s], 3);
+          umma_commit_pair(&ctrl.acc_full[b], 3);
+        }
+      }
+    }
+  } else {
+    setmaxnreg_inc<232>();     // 256 x 232 + 128 x 40 = 384 x 168, the registers of the launch
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + group * COLS;
+    uint8_t* stage = out_buf + (group * 4 + quarter) * (32 * COLS * 2);          // boxes of 32 rows x 64 columns
+    const uint32_t empty_leader0 = map_to_cta(smem_u32(&ctrl.acc_empty[0]), 0), empty_leader1 = map_to_cta(smem_u32(&ctrl.acc_empty[1]), 0);
+    const uint64_t pol = policy_evict_normal();
+    if (p.early) wait_for_previous();
+    int it = 0;
+    for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
+      const int row = (tile % p.tiles_m) * 256 + static_cast<int>(cta_rank) * 128 + quarter * 32 + lane;
+      const int col = (tile / p.tiles_m) * 256 + group * COLS;
+      const bool live = row < p.M && col < p.N;
+      const float* sx = p.sx + static_cast<long long>(live ? row : 0) * p.sx_row;
+      const float* sw = p.sw + static_cast<long long>(live ? col / 128 : 0) * p.sw_row;
+      // Two blocks ahead, and multiplied only when the product is wanted.  (Four at a time in a loop unrolled by four, or
+      // fed by the two idle warps through shared memory: 250 and 255 us instead of 228 for 4096 x 14336 x 4096.)
+      float2 s0 = make_float2(0.0f, 0.0f), s1 = s0;
+      if (live) {
+        s0 = make_float2(*sx, *sw);
+        if (p.KB > 1) s1 = make_float2(sx[p.sx_col], sw[p.sw_col]);
+        sx += 2 * p.sx_col;
+        sw += 2 * p.sw_col;
+      }
+      float2 acc[COLS / 2];
+#pragma unroll
+      for (int j = 0; j < COLS / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+      for (int kb = 0; kb < p.KB; ++kb, ++it) {
+        const int b = it & 1;
+        const float s = s0.x * s0.y;
+        s0 = s1;
+        if (live && kb + 2 < p.KB) {
+          s1 = make_float2(*sx, *sw);
+          sx += p.sx_col;
+          sw += p.sw_col;
+        }
+        bool ok = mbar_wait(&ctrl.acc_full[b], (it >> 1) & 1, abort_word, ERR_ACC_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) goto done;
+        tc_fence_after();
+        const uint32_t ta = lane_addr + b * 256;
+        // two fetches in flight: each is asked for again as soon as its columns have been added
+        uint32_t r0[STEP], r1[STEP];
+        tmem_ld_32x16(ta, r0);
+        tmem_ld_32x16(ta + STEP, r1);
+#pragma unroll
+        for (int c = 0; c < COLS; c += 2 * STEP) {
+          tmem_ld_wait();
+          if (c + 2 * STEP >= COLS) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(b ? empty_leader1 : empty_leader0);
+          }
+          add_scaled(acc, c / 2, r0, s);
+          if (c + 2 * STEP < COLS) tmem_ld_32x16(ta + c + 2 * STEP, r0);
+          add_scaled(acc, c / 2 + STEP / 2, r1, s);
+          if (c + 2 * STEP < COLS) tmem_ld_32x16(ta + c + 3 * STEP, r1);
+        }
+      }
+      if (p.wide) {
+        if (lane == 0) tma_store_wait_read<0>();                       // the last tile's store has left the staging tile
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < COLS / 8; ++j) {
+          // columns 8j .. 8j + 7: box j / 8, 16-byte piece j % 8 of the row's 128 bytes
+          uint8_t* dst = stage + (j >> 3) * 4096 + lane * 128;
+          *reinterpret_cast<uint4*>(dst + (((j & 7) ^ (lane & 7)) << 4)) =
+              make_uint4(pack_bf16(acc[4 * j].x, acc[4 * j].y), pack_bf16(acc[4 * j + 1].x, acc[4 * j + 1].y),
+                         pack_bf16(acc[4 * j + 2].x, acc[4 * j + 2].y), pack_bf16(acc[4 * j + 3].x, acc[4 * j + 3].y));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (row < p.M) {                                             // lane 0: the warp's first row
+#pragma unroll
+            for (int c = 0; c < COLS; c += 64)
+              if (col + c < p.N) tma_store_2d(&tm_out, stage + c * 64, col + c, row, pol);
+          }
+          tma_store_commit();
+        }
+        __syncwarp();
+      } else if (live) {
+        __nv_bfloat16* dst = p.y + static_cast<long long>(row) * p.ld_y + col;
+#pragma unroll
+        for (int j = 0; j < COLS; ++j)
+          if (col + j < p.N) dst[j] = __float2bfloat16_rn(j & 1 ? acc[j / 2].y : acc[j / 2].x);
+      }
+    }
+    if (lane == 0) tma_store_wait_all<0>();
+  }
+
+done:
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_word != 0) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 400000) __nanosleep(1000);
+    if (threadIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, 0, *abort_word);
+    __syncthreads();
+  }
+  cluster_sync_all();          // the peer's shared memory and barriers stay valid until both are done
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& ty, const Params& p, int pairs, int device,
+                  cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  const int rc = allow_smem(fp8_pair_kernel, SMEM, done, device);
+  if (rc != FORGE_OK) return rc;
+  Launch l(2 * pairs, THREADS, SMEM, 2, p.early, stream);
+  cudaError_t e = cudaLaunchKernelEx(&l.cfg, fp8_pair_kernel, tx, tw, ty, p);
+  if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "fp8 product launch: %s", cudaGetErrorString(e));
+  return FORGE_OK;
+}
+}  // namespace pair
 
 }  // namespace fp8
 }  // namespace forge
@@ -479,29 +811,24 @@ extern "C" int forge_fp8_quantize(const ForgeFp8QuantizeArgs* args, void* cuda_s
   return FORGE_OK;
 }
 
-extern "C" int forge_fp8_product(const ForgeFp8ProductArgs* args, void* cuda_stream) {
-  if (args == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_fp8_product: args is NULL");
-  const ForgeFp8ProductArgs& a = *args;
-  if (a.M < 0 || a.N < 0 || a.K < 0) return fail(FORGE_ERR_INVALID_ARG, "forge_fp8_product: negative dimension");
+static int check_product(const ForgeFp8ProductArgs& a, const char* what) {
+  if (a.M < 0 || a.N < 0 || a.K < 0) return fail(FORGE_ERR_INVALID_ARG, "%s: negative dimension", what);
   if (a.M == 0 || a.N == 0) return FORGE_OK;
-  if (a.K < 1) return fail(FORGE_ERR_SHAPE, "forge_fp8_product: K must be at least 1");
-  if (a.M > 0x7fffff00ll || a.N > 0x7fffff00ll || a.K > 0x7fffff00ll) return fail(FORGE_ERR_SHAPE, "forge_fp8_product: dimension too large");
+  if (a.K < 1) return fail(FORGE_ERR_SHAPE, "%s: K must be at least 1", what);
+  if (a.M > 0x7fffff00ll || a.N > 0x7fffff00ll || a.K > 0x7fffff00ll) return fail(FORGE_ERR_SHAPE, "%s: dimension too large", what);
   if (a.x_codes == nullptr || a.x_scales == nullptr || a.w_codes == nullptr || a.w_scales == nullptr || a.y == nullptr)
-    return fail(FORGE_ERR_INVALID_ARG, "forge_fp8_product: null pointer");
+    return fail(FORGE_ERR_INVALID_ARG, "%s: null pointer", what);
   if (!aligned16(a.x_codes) || !aligned16(a.w_codes) || a.ld_x % 16 || a.ld_w % 16)
-    return fail(FORGE_ERR_ALIGNMENT, "forge_fp8_product: codes must start on 16-byte boundaries and have row pitches that are multiples of 16");
-  if (a.ld_x < a.K || a.ld_w < a.K || a.ld_y < a.N) return fail(FORGE_ERR_SHAPE, "forge_fp8_product: row pitch smaller than the row");
-  if (reinterpret_cast<uintptr_t>(a.y) % 2) return fail(FORGE_ERR_ALIGNMENT, "forge_fp8_product: y is not element-aligned");
+    return fail(FORGE_ERR_ALIGNMENT, "%s: codes must start on 16-byte boundaries and have row pitches that are multiples of 16", what);
+  if (a.ld_x < a.K || a.ld_w < a.K || a.ld_y < a.N) return fail(FORGE_ERR_SHAPE, "%s: row pitch smaller than the row", what);
+  if (reinterpret_cast<uintptr_t>(a.y) % 2) return fail(FORGE_ERR_ALIGNMENT, "%s: y is not element-aligned", what);
+  return FORGE_OK;
+}
+
+static int run_product(const ForgeFp8ProductArgs& a, bool early, cudaStream_t stream) {
   const DeviceInfo* di = current_device_info();
   if (di == nullptr) return FORGE_ERR_CUDA;
   if (di->cc_major != 10) return fail(FORGE_ERR_DEVICE, "device %d is sm_%d%d, not sm_100", di->device, di->cc_major, di->cc_minor);
-
-  const int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-  CUtensorMap tw, tx;
-  int rc = encode_tmap_2d(&tw, a.w_codes, 1, false, a.N, a.K, a.ld_w, fp8::BK, 128, 128);
-  if (rc != FORGE_OK) return rc;
-  rc = encode_tmap_2d(&tx, a.x_codes, 1, false, a.M, a.K, a.ld_x, fp8::BK, nt, 128);
-  if (rc != FORGE_OK) return rc;
   fp8::Params p;
   p.sx = a.x_scales; p.sw = a.w_scales;
   p.y = static_cast<__nv_bfloat16*>(a.y);
@@ -509,21 +836,69 @@ extern "C" int forge_fp8_product(const ForgeFp8ProductArgs* args, void* cuda_str
   p.ld_y = a.ld_y;
   p.M = static_cast<int>(a.M); p.N = static_cast<int>(a.N);
   p.KB = static_cast<int>((a.K + fp8::BK - 1) / fp8::BK);
-  p.tiles_m = static_cast<int>((a.M + nt - 1) / nt);
   p.wide = aligned16(a.y) && a.ld_y % 8 == 0;
+  p.early = early;
   p.status = a.status;
+
+  const int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  p.tiles_m = static_cast<int>((a.M + nt - 1) / nt);
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * ((a.N + 127) / 128);
   // K is cut until the CTAs fill the GPU once (two per SM up to 64 tokens), each with two K blocks at least
   const int64_t slots = static_cast<int64_t>(di->sm_count) * (nt == 128 ? 1 : 2);
   p.split = 1;
-  while (p.split < 8 && tiles * p.split * 2 <= slots && p.KB >= p.split * 4) p.split *= 2;
+  // (clusters of eight leave a few SMs of every GPC unused: count on three quarters)
+  while (p.split < 8 && tiles * p.split * 2 <= (p.split == 4 ? slots * 3 / 4 : slots) && p.KB >= p.split * 4) p.split *= 2;
   if (tiles * p.split > 0x7fffffffll) return fail(FORGE_ERR_SHAPE, "forge_fp8_product: too many tiles");
-  const int ctas = static_cast<int>(tiles * p.split);
-  cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-  switch (nt) {
-    case 16: return fp8::launch_product<16>(tw, tx, p, ctas, s);
-    case 32: return fp8::launch_product<32>(tw, tx, p, ctas, s);
-    case 64: return fp8::launch_product<64>(tw, tx, p, ctas, s);
-    default: return fp8::launch_product<128>(tw, tx, p, ctas, s);
+
+  // Pairs of CTAs where they need fewer rounds of K blocks over the GPU than the tiles of 128 x 128, a round taking about
+  // as long in both (0.55 us).  With K = 4096, pairs / tiles: 256 x 14336 23.5 / 42 us, 512 x 14336 39 / 78,
+  // 4096 x 14336 228 / 478, 512 x 4096 22 / 23, 512 x 1024 20 / 13.5 (K cut in four), 128 x 4096 21 / 14.
+  const int64_t pair_tiles = ((a.M + 255) / 256) * ((a.N + 255) / 256), pair_slots = di->sm_count / 2;
+  const int64_t pair_time = (pair_tiles + pair_slots - 1) / pair_slots * p.KB;
+  const int64_t tile_time = (tiles * p.split + slots - 1) / slots * ((p.KB + p.split - 1) / p.split);
+  const bool pairs = nt == 128 && pair_time < tile_time;
+  CUtensorMap tw, tx, ty;
+  int rc = encode_tmap_2d(&tw, a.w_codes, 1, false, a.N, a.K, a.ld_w, fp8::BK, 128, 128);
+  if (rc != FORGE_OK) return rc;
+  rc = encode_tmap_2d(&tx, a.x_codes, 1, false, a.M, a.K, a.ld_x, fp8::BK, nt, 128);
+  if (rc != FORGE_OK) return rc;
+  if (pairs) {
+    ty = tx;                                   // not used without aligned rows
+    if (p.wide) {
+      rc = encode_tmap_2d(&ty, a.y, 2, true, a.M, a.N, a.ld_y, 64, 32, 128);
+      if (rc != FORGE_OK) return rc;
+    }
+    p.tiles_m = static_cast<int>((a.M + 255) / 256);
+    p.split = 1;
+    return fp8::pair::launch(tx, tw, ty, p, static_cast<int>(std::min<int64_t>(pair_tiles, pair_slots)), di->device, stream);
   }
+  const int ctas = static_cast<int>(tiles * p.split);
+  switch (nt) {
+    case 16: return fp8::launch_product<16>(tw, tx, p, ctas, di->device, stream);
+    case 32: return fp8::launch_product<32>(tw, tx, p, ctas, di->device, stream);
+    case 64: return fp8::launch_product<64>(tw, tx, p, ctas, di->device, stream);
+    default: return fp8::launch_product<128>(tw, tx, p, ctas, di->device, stream);
+  }
+}
+
+extern "C" int forge_fp8_product(const ForgeFp8ProductArgs* args, void* cuda_stream) {
+  if (args == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_fp8_product: args is NULL");
+  const int rc = check_product(*args, "forge_fp8_product");
+  if (rc != FORGE_OK || args->M == 0 || args->N == 0) return rc;
+  return run_product(*args, false, static_cast<cudaStream_t>(cuda_stream));
+}
+
+extern "C" int forge_fp8_linear(const ForgeFp8QuantizeArgs* x, const ForgeFp8ProductArgs* product, void* cuda_stream) {
+  if (x == nullptr || product == nullptr) return fail(FORGE_ERR_INVALID_ARG, "forge_fp8_linear: null pointer");
+  const ForgeFp8ProductArgs& a = *product;
+  if (x->block_rows != 1 || x->codes_t != nullptr || x->rows != a.M || x->cols != a.K || x->codes != a.x_codes || x->ld_codes != a.ld_x ||
+      x->scales != a.x_scales || a.x_scale_row != (a.K + 127) / 128 || a.x_scale_col != 1)
+    return fail(FORGE_ERR_INVALID_ARG, "forge_fp8_linear: the quantiser's output is not the product's X");
+  int rc = check_product(a, "forge_fp8_linear");
+  if (rc != FORGE_OK || a.M == 0 || a.N == 0) return rc;
+  rc = forge_fp8_quantize(x, cuda_stream);
+  if (rc != FORGE_OK) return rc;
+  // The product may start under the quantiser: what it reads before that has ended (the weight) was written before
+  // the quantiser was launched, and the quantiser was launched after all work in front of it.
+  return run_product(a, true, static_cast<cudaStream_t>(cuda_stream));
 }

@@ -290,7 +290,6 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ws
   q.codes = codes;
   q.ld_codes = pitch;
   q.scales = scales;
-  check(forge_fp8_quantize(&q, stream), "forge_fp8_quantize");
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;
   at::Tensor y = at::empty(shape, opt.dtype(at::kBFloat16));
@@ -303,7 +302,7 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ws
   a.x_scale_row = kb; a.x_scale_col = 1;
   a.w_scale_row = ws.stride(0); a.w_scale_col = ws.stride(1);
   a.status = g_status[dev];
-  check(forge_fp8_product(&a, stream), "forge_fp8_product");
+  check(forge_fp8_linear(&q, &a, stream), "forge_fp8_linear");
   return y;
 }
 

@@ -435,6 +435,10 @@ typedef struct ForgeFp8ProductArgs {
 } ForgeFp8ProductArgs;
 int forge_fp8_product(const ForgeFp8ProductArgs* args, void* cuda_stream);
 
+/* forge_fp8_quantize of x by rows and forge_fp8_product of what it wrote, with the start of the second overlapped with
+ * the end of the first.  product->x_codes, ld_x, x_scales and scale strides are those of the quantiser's output. */
+int forge_fp8_linear(const ForgeFp8QuantizeArgs* x, const ForgeFp8ProductArgs* product, void* cuda_stream);
+
 /* Bytes of optimizer state the allocator must provide for a (V, H) parameter: the moment arrays
  * and, separately, the scale arrays (src/fused_grad_optimizer/state.py:95-130). */
 int forge_state_bytes(int32_t optimizer, int32_t mode, int64_t V, int64_t H, int32_t qblock,

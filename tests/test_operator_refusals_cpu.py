@@ -134,6 +134,21 @@ def test_product_refuses(kw, code):
     assert _lib.load().forge_fp8_product(None, None) == _lib.FORGE_ERR_INVALID_ARG
 
 
+@pytest.mark.parametrize("xkw,pkw,code", [
+    (dict(block_rows=128), {}, _lib.FORGE_ERR_INVALID_ARG), (dict(rows=5), {}, _lib.FORGE_ERR_INVALID_ARG),
+    (dict(cols=128), {}, _lib.FORGE_ERR_INVALID_ARG), (dict(codes=P + 256), {}, _lib.FORGE_ERR_INVALID_ARG),
+    (dict(ld_codes=272), {}, _lib.FORGE_ERR_INVALID_ARG), ({}, dict(x_scale_row=1, x_scale_col=4), _lib.FORGE_ERR_INVALID_ARG),
+    (dict(scales=P + 64), {}, _lib.FORGE_ERR_INVALID_ARG), ({}, dict(y=None), _lib.FORGE_ERR_INVALID_ARG),
+    ({}, dict(ld_w=264), _lib.FORGE_ERR_ALIGNMENT), (dict(rows=0), dict(M=0), 0)])
+def test_linear_refuses(xkw, pkw, code):
+    x = dict(x=P, rows=4, cols=256, ld_x=256, dtype=_lib.DT_BF16, block_rows=1, codes=P, ld_codes=256, scales=P)
+    base = dict(x_codes=P, x_scales=P, w_codes=P, w_scales=P, y=P, M=4, N=128, K=256, ld_x=256, ld_w=256, ld_y=128,
+                x_scale_row=2, x_scale_col=1, w_scale_row=2, w_scale_col=1)
+    a, b = fill(_lib.ForgeFp8QuantizeArgs, x, xkw), fill(_lib.ForgeFp8ProductArgs, base, pkw)
+    assert _lib.load().forge_fp8_linear(ctypes.byref(a), ctypes.byref(b), None) == code
+    assert _lib.load().forge_fp8_linear(None, ctypes.byref(b), None) == _lib.FORGE_ERR_INVALID_ARG
+
+
 def test_wrappers_refuse_cpu_tensors():
     from forge_b200.fp8 import Fp8Weight, fp8_linear, fp8_matmul, quantize_fp8
     from forge_b200.loss import logprob_parts, token_logprobs
