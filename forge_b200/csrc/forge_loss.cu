@@ -28,6 +28,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "forge_host.h"
@@ -712,11 +713,14 @@ static Params make_params(const ForgeLogprobsArgs& a) {
 }
 
 template <int DT, bool TOP>
-static int launch_forward(const Params& p, long long rows, int cs, cudaStream_t stream) {
+static int launch_forward(const Params& p, long long rows, int cs, int device, cudaStream_t stream) {
   auto* fn = logprobs_kernel<DT, TOP>;
-  if (cs > 8) {
+  static std::atomic<uint64_t> allowed{0};             // devices on which clusters of sixteen have been allowed
+  const uint64_t bit = 1ull << (device & 63);
+  if (cs > 8 && !(allowed.load(std::memory_order_relaxed) & bit)) {
     cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "logprobs: cluster attribute: %s", cudaGetErrorString(e));
+    allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * cs));
@@ -764,8 +768,8 @@ extern "C" int forge_logprobs_forward(const ForgeLogprobsArgs* args, void* cuda_
   const loss::Params p = loss::make_params(a);
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   if (a.dtype == FORGE_DT_BF16)
-    return a.top_k > 0 ? loss::launch_forward<DT_BF16, true>(p, a.rows, cs, s) : loss::launch_forward<DT_BF16, false>(p, a.rows, cs, s);
-  return a.top_k > 0 ? loss::launch_forward<DT_F32, true>(p, a.rows, cs, s) : loss::launch_forward<DT_F32, false>(p, a.rows, cs, s);
+    return a.top_k > 0 ? loss::launch_forward<DT_BF16, true>(p, a.rows, cs, di->device, s) : loss::launch_forward<DT_BF16, false>(p, a.rows, cs, di->device, s);
+  return a.top_k > 0 ? loss::launch_forward<DT_F32, true>(p, a.rows, cs, di->device, s) : loss::launch_forward<DT_F32, false>(p, a.rows, cs, di->device, s);
 }
 
 extern "C" int forge_logprobs_join(const ForgeLogprobsArgs* args, const float* stats, const uint64_t* keys, int32_t parts,

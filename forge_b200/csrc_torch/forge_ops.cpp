@@ -3,14 +3,14 @@
 // norm weights of a decoder).  Every function returns None for arguments that are not of the plain form it handles
 // (another dtype or layout, a wrong shape, CPU tensors); the Python wrappers then take over, which check, copy or refuse.
 // Both paths issue the same library calls.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
-#include <cmath>
-#include <unordered_set>
+#include <array>
 #include <vector>
 
 #include "../../include/forge_b200.h"
@@ -70,25 +70,29 @@ ForgeLogprobsArgs loss_args(const at::Tensor& x, const Rows& r, const at::Tensor
   return a;
 }
 
-// {logprobs, entropy, lse, top_logprobs, top_ids}
-std::vector<at::Tensor> loss_forward(const at::Tensor& x, const at::Tensor& t, int64_t top_k, double temperature, int64_t ignore) {
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
+}
+
+// {logprobs, entropy, lse (if it is wanted), top_logprobs, top_ids}
+std::array<at::Tensor, 5> loss_forward(const at::Tensor& x, const at::Tensor& t, int64_t top_k, double temperature, int64_t ignore,
+                                       bool with_lse) {
   Rows r;
   as_rows(x, r);
   const int dev = x.get_device();
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
   ForgeLogprobsArgs a = loss_args(x, r, t, top_k, temperature, ignore);
   const auto lead = x.sizes().slice(0, x.dim() - 1);
-  const auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
-  std::vector<at::Tensor> out(5);
-  for (int i = 0; i < 3; ++i) out[i] = at::empty(lead, f32);
+  std::array<at::Tensor, 5> out;
+  for (int i = 0; i < (with_lse ? 3 : 2); ++i) out[i] = empty(lead, at::kFloat, x);
   a.logprobs = static_cast<float*>(out[0].data_ptr());
   a.entropy = static_cast<float*>(out[1].data_ptr());
-  a.lse = static_cast<float*>(out[2].data_ptr());
+  a.lse = with_lse ? static_cast<float*>(out[2].data_ptr()) : nullptr;
   if (top_k > 0) {
-    std::vector<int64_t> shape(lead.begin(), lead.end());
+    c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end());
     shape.push_back(top_k);
-    out[3] = at::empty(shape, f32);
-    out[4] = at::empty(shape, f32.dtype(at::kLong));
+    out[3] = empty(shape, at::kFloat, x);
+    out[4] = empty(shape, at::kLong, x);
     a.top_logprobs = static_cast<float*>(out[3].data_ptr());
     a.top_ids = static_cast<int64_t*>(out[4].data_ptr());
   }
@@ -100,7 +104,7 @@ class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
  public:
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& t, int64_t top_k, double temperature,
                                int64_t ignore) {
-    auto out = loss_forward(x, t, top_k, temperature, ignore);
+    auto out = loss_forward(x, t, top_k, temperature, ignore, true);
     ctx->save_for_backward({x, t, out[2], out[1]});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore"] = ignore;
@@ -129,7 +133,7 @@ class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
       ForgeLogprobsArgs a = loss_args(x, r, t, 0, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt());
       a.lse = static_cast<float*>(const_cast<void*>(saved[2].const_data_ptr()));
       a.entropy = static_cast<float*>(const_cast<void*>(saved[3].const_data_ptr()));
-      dx = at::empty(x.sizes(), x.options().requires_grad(false));
+      dx = empty(x.sizes(), x.scalar_type(), x);
       check(forge_logprobs_backward(&a, gr[0].defined() ? static_cast<const float*>(gr[0].const_data_ptr()) : nullptr,
                                     gr[1].defined() ? static_cast<const float*>(gr[1].const_data_ptr()) : nullptr, dx.data_ptr(), r.vocab,
                                     stream_of(dev)),
@@ -156,7 +160,7 @@ py::object token_logprobs(const at::Tensor& x, const c10::optional<at::Tensor>& 
     const auto out = TokenLogprobsFn::apply(x, t, top_k, temperature, ignore);
     return py::make_tuple(wrap(out[0]), wrap(out[1]), top_k ? wrap(out[2]) : none, top_k ? wrap(out[3]) : none);
   }
-  const auto out = loss_forward(x, t, top_k, temperature, ignore);
+  const auto out = loss_forward(x, t, top_k, temperature, ignore, false);
   return py::make_tuple(wrap(out[0]), wrap(out[1]), top_k ? wrap(out[3]) : none, top_k ? wrap(out[4]) : none);
 }
 
@@ -175,6 +179,30 @@ bool unpack(const py::handle& seq, std::vector<const at::Tensor*>& out) {
   }
   return true;
 }
+
+// a set of addresses in one flat table
+class PointerSet {
+ public:
+  explicit PointerSet(size_t most) {
+    while ((size_t(1) << bits_) < 2 * most) ++bits_;
+    table_.assign(size_t(1) << bits_, nullptr);
+  }
+  // false if it was there already
+  bool insert(const void* p) {
+    const size_t mask = table_.size() - 1;
+    for (size_t i = (reinterpret_cast<uintptr_t>(p) * 0x9E3779B97F4A7C15ull) >> (64 - bits_);; i = (i + 1) & mask) {
+      if (table_[i] == p) return false;
+      if (table_[i] == nullptr) {
+        table_[i] = p;
+        return true;
+      }
+    }
+  }
+
+ private:
+  int bits_ = 4;
+  std::vector<const void*> table_;
+};
 
 bool plain(const at::Tensor& t, int dev) {
   return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous();
@@ -204,8 +232,7 @@ py::object multi_adamw(const py::object& params, const py::object& grads, const 
     return none;
   }
   std::vector<ForgeMultiItem> items(n);
-  std::unordered_set<const void*> seen;
-  seen.reserve(3 * n);
+  PointerSet seen(3 * n);
   for (size_t i = 0; i < n; ++i) {
     const int64_t num = p[i]->numel();
     if (!plain(*p[i], dev) || !plain(*g[i], dev) || !plain(*m[i], dev) || !plain(*v[i], dev) || !float_type(*p[i]) || !float_type(*g[i]) ||
@@ -227,7 +254,7 @@ py::object multi_adamw(const py::object& params, const py::object& grads, const 
       it.m_scale = static_cast<float*>(ms[i]->mutable_data_ptr());
       it.v_scale = static_cast<float*>(vs[i]->mutable_data_ptr());
     }
-    if (num > 0 && (!seen.insert(it.param).second || !seen.insert(it.m).second || !seen.insert(it.v).second)) return none;
+    if (num > 0 && !(seen.insert(it.param) && seen.insert(it.m) && seen.insert(it.v))) return none;
   }
   ForgeMultiArgs a = {};
   if (grad_coef.has_value() && grad_coef->defined()) {
@@ -241,9 +268,8 @@ py::object multi_adamw(const py::object& params, const py::object& grads, const 
     std::vector<ForgeNormItem> gi(n);
     for (size_t i = 0; i < n; ++i) gi[i] = ForgeNormItem{items[i].grad, items[i].numel, items[i].grad_dtype, 0};
     const size_t bytes = forge_multi_norm_scratch_bytes(gi.data(), static_cast<int32_t>(n));
-    const auto f32 = p[0]->options().dtype(at::kFloat).requires_grad(false);
-    out = at::empty({2}, f32);
-    scratch = at::empty({static_cast<int64_t>(bytes / 4 + 2)}, f32);
+    out = empty({2}, at::kFloat, *p[0]);
+    scratch = empty({static_cast<int64_t>(bytes + 8)}, at::kByte, *p[0]);
     float* o = static_cast<float*>(out.data_ptr());
     check(forge_multi_norm(gi.data(), static_cast<int32_t>(n), max_norm, o, o + 1, scratch.data_ptr(), bytes, stream), "forge_multi_norm");
     a.grad_coef = o + 1;
@@ -277,9 +303,8 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ws
   const int64_t K = w.size(1), N = w.size(0), pitch = (K + 15) / 16 * 16, kb = blocks(K);
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
   void* stream = stream_of(dev);
-  const auto opt = x.options().requires_grad(false);
   // codes and scales of this call in one allocation: rows of `pitch` bytes, then M x kb floats
-  at::Tensor buf = at::empty({M * pitch + M * kb * 4}, opt.dtype(at::kByte));
+  at::Tensor buf = empty({M * pitch + M * kb * 4}, at::kByte, x);
   uint8_t* codes = static_cast<uint8_t*>(buf.data_ptr());
   float* scales = reinterpret_cast<float*>(codes + M * pitch);
   ForgeFp8QuantizeArgs q = {};
@@ -290,9 +315,9 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ws
   q.codes = codes;
   q.ld_codes = pitch;
   q.scales = scales;
-  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;
-  at::Tensor y = at::empty(shape, opt.dtype(at::kBFloat16));
+  at::Tensor y = empty(shape, at::kBFloat16, x);
   ForgeFp8ProductArgs a = {};
   a.x_codes = codes; a.x_scales = scales;
   a.w_codes = w.const_data_ptr(); a.w_scales = static_cast<const float*>(ws.const_data_ptr());
@@ -354,14 +379,12 @@ py::object quantize(const at::Tensor& x, int64_t block_rows, bool transposed) {
   const int dev = x.get_device();
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
   const int64_t R = x.size(0), C = x.size(1), sr = block_rows == 1 ? R : blocks(R), sc = blocks(C);
-  const auto opt = x.options().requires_grad(false);
-  const auto f32 = opt.dtype(at::kFloat), f8 = opt.dtype(at::kFloat8_e4m3fn);
   auto codes = [&](int64_t r, int64_t c) {
     const int64_t pitch = (c + 15) / 16 * 16;
-    at::Tensor t = at::empty({r, pitch}, f8);
+    at::Tensor t = empty({r, pitch}, at::kFloat8_e4m3fn, x);
     return pitch == c ? t : t.narrow(1, 0, c);
   };
-  at::Tensor q = codes(R, C), s = at::empty({sr, sc}, f32), qt, st;
+  at::Tensor q = codes(R, C), s = empty({sr, sc}, at::kFloat, x), qt, st;
   ForgeFp8QuantizeArgs a = {};
   a.x = x.const_data_ptr();
   a.rows = R; a.cols = C; a.ld_x = C;
@@ -372,7 +395,7 @@ py::object quantize(const at::Tensor& x, int64_t block_rows, bool transposed) {
   a.scales = static_cast<float*>(s.data_ptr());
   if (transposed) {
     qt = codes(C, R);
-    st = at::empty({sc, sr}, f32);
+    st = empty({sc, sr}, at::kFloat, x);
     a.codes_t = qt.data_ptr();
     a.ld_codes_t = (R + 15) / 16 * 16;
     a.scales_t = static_cast<float*>(st.data_ptr());
