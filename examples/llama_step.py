@@ -4,7 +4,9 @@ Qwen3-32B with fp8 moments; batch 1 x 512 tokens).
 Builds a Llama-3.1-8B (or Qwen3-32B) architecture from its config with random weights -- no
 checkpoint, no dataset: tokens are uniform over the vocabulary -- swaps every ``nn.Linear`` for
 ``FusedLinear.from_linear`` (same recipe as the reference's README), leaves embeddings and norms to a
-regular ``torch.optim.AdamW``, and reports the median step time and the peak device memory.
+regular ``torch.optim.AdamW`` (or, ``--rest-state``, to ``MultiTensorAdamW``), and reports the median step time and the
+peak device memory.  ``--forge-loss`` forms the loss with ``token_logprobs`` instead of the model's own cross entropy,
+``--fp8-products`` the forward products and input gradients in e4m3.
 
     python examples/llama_step.py --model llama3.1-8b --state bf16 --steps 20
     python examples/llama_step.py --model llama3.1-8b --baseline      # vanilla fused torch AdamW
@@ -59,6 +61,21 @@ def swap_linears(module, state_mode, use_dgrad):
     return n
 
 
+def rest_optimizer(args, params):
+    """The optimizer of the parameters that are not fused linears."""
+    if args.rest_state is None:
+        return torch.optim.AdamW(params, lr=1e-4, weight_decay=0.01, fused=True, capturable=args.graph)
+    from forge_b200.multi_tensor import MultiTensorAdamW
+    opt = MultiTensorAdamW(params, lr=1e-4, weight_decay=0.01, state_mode=args.rest_state)
+    return opt.enable_device_hyper() if args.graph else opt
+
+
+def pre_step(opt):
+    """Hyper-parameters of the coming step to the device, where the optimizer reads them from there."""
+    if getattr(opt, "reads_device_hyper", False):
+        opt.pre_step()
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--model", default="llama3.1-8b")
@@ -88,6 +105,12 @@ def main():
                     help="--fused-scatter: 'gathered' keeps q/k/v and gate/up (replicated input) on library GEMMs + NCCL "
                          "all-reduce; 'all' also forms their input gradient with one GEMM launch per set whose tiles go to every rank")
     ap.add_argument("--torch-norm", action="store_true", help="--tp: RMSNorm as torch ops instead of the library's kernels")
+    ap.add_argument("--forge-loss", action="store_true", help="next-token loss and its gradient through the library's kernels "
+                    "(forge_b200.loss) instead of the model's own cross entropy (--tp: instead of torch ops)")
+    ap.add_argument("--rest-state", choices=("f32", "bf16", "int8", "fp8_block"), default=None,
+                    help="embeddings and norms through MultiTensorAdamW with moments of this kind instead of torch.optim.AdamW")
+    ap.add_argument("--fp8-products", action="store_true",
+                    help="single GPU: forward products and input gradients of the fused linears in e4m3 with block scales")
     ap.add_argument("--no-group", action="store_true", help="one launch per linear instead of one per decoder layer")
     args = ap.parse_args()
     if args.tp:
@@ -120,10 +143,11 @@ def main():
         manager = FusedOptimizerManager(model)
         if not args.no_group:
             manager.group_updates("layer")
+        if args.fp8_products:
+            manager.use_fp8_products()
         if args.graph:
             manager.enable_device_hyper(dev)
-        opt = torch.optim.AdamW(manager.get_non_fused_params(), lr=1e-4, weight_decay=0.01, fused=True,
-                                capturable=args.graph)
+        opt = rest_optimizer(args, manager.get_non_fused_params())
 
     torch.cuda.reset_peak_memory_stats(dev)
     times, losses = [], []
@@ -131,7 +155,12 @@ def main():
     static_loss = torch.zeros((), device=dev)
 
     def one_step(ids):
-        loss = model(input_ids=ids, labels=ids).loss
+        if args.forge_loss:
+            from forge_b200.loss import token_logprobs
+            logits = model(input_ids=ids).logits
+            loss = -token_logprobs(logits[:, :-1], ids[:, 1:]).logprobs.mean()
+        else:
+            loss = model(input_ids=ids, labels=ids).loss
         loss.backward()
         opt.step()
         opt.zero_grad(set_to_none=True)
@@ -155,6 +184,7 @@ def main():
             static_ids.copy_(ids)
             if manager is not None:
                 manager.pre_step(lr=1e-4, weight_decay=0.01)
+            pre_step(opt)
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 static_loss.copy_(one_step(static_ids).detach())
@@ -166,6 +196,7 @@ def main():
         t0 = time.perf_counter()
         if manager is not None:
             manager.pre_step(lr=1e-4, weight_decay=0.01)
+        pre_step(opt)
         if graph is not None:
             static_ids.copy_(ids)
             graph.replay()
@@ -192,6 +223,7 @@ def main():
         "steps": args.steps, "peak_hbm_gb": torch.cuda.max_memory_allocated(dev) / 1e9, "memory": mem,
         "first_loss": losses[0], "last_loss": losses[-1], "device_status": status,
         "forge_dgrad": bool(args.forge_dgrad), "fuse_norm": bool(args.fuse_norm and not args.baseline),
+        "forge_loss": bool(args.forge_loss), "rest_state": args.rest_state, "fp8_products": bool(args.fp8_products and not args.baseline),
         "cuda_graph": bool(args.graph), "data": "synthetic uniform tokens, random init",
     }))
 
@@ -216,9 +248,10 @@ def run_tp(args):
     cfg = dict(CONFIGS[args.model])
     if args.layers:
         cfg["layers"] = args.layers
+    from examples import tp_model
     if args.torch_norm:
-        from examples import tp_model
         tp_model.RMSNorm.library_kernels = False
+    tp_model.TPDecoder.library_loss = args.forge_loss
     model = TPDecoder(cfg, state_mode=args.state, device=dev).train()
     if args.fused_scatter and world > 1:
         model.use_fused_scatter(args.seq, replicated_sets=args.fused_scatter_sets == "all")
@@ -229,7 +262,7 @@ def run_tp(args):
         manager.group_updates("layer")
     if args.graph:
         manager.enable_device_hyper(dev)
-    opt = torch.optim.AdamW(manager.get_non_fused_params(), lr=1e-4, weight_decay=0.01, fused=True, capturable=args.graph)
+    opt = rest_optimizer(args, manager.get_non_fused_params())
     head_norms = model.head_sharded_norm_params()
     n_local = sum(p.numel() for p in model.parameters())
     n_sharded = sum(m.weight.numel() for m in manager._fused_modules)
@@ -263,6 +296,7 @@ def run_tp(args):
         if args.graph and graph is None and step == 2:
             static_ids.copy_(ids)
             manager.pre_step(lr=1e-4, weight_decay=0.01)
+            pre_step(opt)
             try:
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph):
@@ -283,6 +317,7 @@ def run_tp(args):
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
         manager.pre_step(lr=1e-4, weight_decay=0.01)
+        pre_step(opt)
         if graph is not None:
             static_ids.copy_(ids)
             graph.replay()
@@ -314,7 +349,8 @@ def run_tp(args):
             "device_status": int(stats[2].item()), "cuda_graph": bool(graph is not None),
             "grouped_launches": not args.no_group, "forge_dgrad": bool(args.forge_dgrad),
             "fused_scatter": (args.fused_scatter_sets if args.fused_scatter and world > 1 else False),
-            "fused_gather": bool(args.fused_gather and world > 1), "library_rmsnorm": not args.torch_norm, "clocks": clocks,
+            "fused_gather": bool(args.fused_gather and world > 1), "library_rmsnorm": not args.torch_norm, "forge_loss": bool(args.forge_loss),
+            "rest_state": args.rest_state, "clocks": clocks,
             "timing": "CUDA events per step, median over steps, max over ranks",
             "data": "synthetic uniform tokens (same on every rank), random init"}))
     sys.stdout.flush()

@@ -221,8 +221,18 @@ class Block(nn.Module):
         return h + _GatherIntoReplicated.apply(d, self.group)
 
 
+def library_cross_entropy(logits_r, targets, v0, vocab, group):
+    """The same mean through ``forge_b200.loss``: one pass over this rank's logits, a few numbers per row gathered, the
+    gradient formed from the logits themselves instead of from a stored fp32 copy of the probabilities."""
+    from forge_b200.loss import token_logprobs
+    group = group if group is not None else dist.group.WORLD
+    return -token_logprobs(logits_r, targets, vocab_start=v0, vocab_total=vocab, group=group).logprobs.mean()
+
+
 class TPDecoder(nn.Module):
     """``cfg``: dict with vocab, hidden, ffn, layers, q_heads, kv_heads, head_dim, eps, rope_theta, qk_norm."""
+
+    library_loss = False        # True: the loss through the library's kernels instead of torch ops
 
     def __init__(self, cfg, group=None, state_mode="bf16", dtype=torch.bfloat16, device=None):
         super().__init__()
@@ -306,7 +316,10 @@ class TPDecoder(nn.Module):
         logits_r = self.lm_head(x)                               # (B, T, vocab / R)
         v0 = self.lm_head.row_start
         flat = logits_r[:, :-1].reshape(-1, logits_r.shape[-1])
-        return _VocabParallelCrossEntropy.apply(flat, ids[:, 1:].reshape(-1), v0, self.group)
+        targets = ids[:, 1:].reshape(-1)
+        if TPDecoder.library_loss:
+            return library_cross_entropy(flat, targets, v0, self.cfg["vocab"], self.group)
+        return _VocabParallelCrossEntropy.apply(flat, targets, v0, self.group)
 
 
 CONFIGS = {

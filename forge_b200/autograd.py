@@ -22,6 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from forge_b200 import kernel as K
+from forge_b200.fp8 import Fp8Weight, fp8_linear
 from forge_b200.state import FusedOptimizerState, OptimizerConfig  # noqa: F401  (re-exported)
 
 # dX through the library's own GEMM (bf16 CUDA operands); plain `grad_output @ weight` otherwise
@@ -42,7 +43,13 @@ class FusedLinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, input, weight, bias, optimizer_state, optimizer_config, is_accumulating,
-                l2_manager, use_fused_backward=True, update_group=None):
+                l2_manager, use_fused_backward=True, update_group=None, fp8_products=False):
+        # fp8_products (no reference counterpart): both products in e4m3; the transposed codes of the weight as it is now wait
+        # for the backward pass
+        ctx.fp8_weight = None
+        if fp8_products:
+            w8 = Fp8Weight.from_weight(weight, transposed=ctx.needs_input_grad[0])
+            ctx.fp8_weight = (w8.codes_t, w8.scales_t)
         # update_group (no reference counterpart): a LayerUpdateGroup that collects the fused updates of
         # several linears and issues them as one launch once every member has reported
         ctx.update_group = update_group
@@ -52,6 +59,8 @@ class FusedLinearFunction(torch.autograd.Function):
         ctx.is_accumulating = is_accumulating
         ctx.l2_manager = l2_manager
         ctx.use_fused_backward = use_fused_backward
+        if fp8_products:
+            return fp8_linear(input.detach(), w8, bias)
         return F.linear(input, weight, bias)
 
     @staticmethod
@@ -60,7 +69,12 @@ class FusedLinearFunction(torch.autograd.Function):
         state, config = ctx.optimizer_state, ctx.optimizer_config
 
         # before any in-place update of `weight` on this stream
-        grad_input = _grad_input(grad_output, weight) if ctx.needs_input_grad[0] else None
+        grad_input = None
+        if ctx.needs_input_grad[0]:
+            if ctx.fp8_weight is not None:
+                grad_input = fp8_linear(grad_output.to(torch.bfloat16), Fp8Weight(*ctx.fp8_weight))
+            else:
+                grad_input = _grad_input(grad_output, weight)
 
         x2d = input.reshape(-1, input.shape[-1])
         dy2d = grad_output.reshape(-1, grad_output.shape[-1])
@@ -83,7 +97,7 @@ class FusedLinearFunction(torch.autograd.Function):
                 _apply_fused(dy2d, x2d, weight, state, config, ctx.l2_manager)
 
         grad_bias = dy2d.sum(0) if bias is not None else None
-        return grad_input, grad_weight, grad_bias, None, None, None, None, None, None
+        return grad_input, grad_weight, grad_bias, None, None, None, None, None, None, None
 
 
 def native_proto(weight, state):

@@ -138,7 +138,7 @@ def _gather_parts(stats, keys, group):
     for t in (stats, keys):
         parts = t.new_empty(world, *t.shape)
         if t.numel():
-            dist.all_gather(list(parts.unbind(0)), t, group=group)
+            dist.all_gather_into_tensor(parts.view(-1), t.reshape(-1), group=group)
         out.append(parts)
     return out
 

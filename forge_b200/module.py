@@ -73,6 +73,8 @@ class FusedLinear(nn.Module):
         self._l2_manager = None
         # False: materialise grad_W with a library GEMM and run the optimizer-only kernel
         self.use_fused_backward = True
+        # see use_fp8_products
+        self.fp8_products = False
         # set by FusedOptimizerManager.group_updates: the launch this module's update is issued with
         self._update_group = None
         # handle of the C++ autograd node (forge_b200.native), created on first use
@@ -122,6 +124,18 @@ class FusedLinear(nn.Module):
     def set_accumulating(self, is_accumulating: bool):
         self._is_accumulating = is_accumulating
 
+    def use_fp8_products(self, on: bool = True):
+        """Form the training forward product and the input gradient in e4m3 with one scale per block of 128
+        (``forge_b200.fp8``): activations and output gradients are quantised by rows, the weight by 128 x 128 blocks, anew in
+        every training forward.  The weight gradient and the update stay the fused kernel's, from the bf16 activations.  Pays
+        from a few thousand tokens per step on (quantising the weight costs two passes over it); between forward and
+        backward the transposed codes are kept, one byte per weight.  Evaluation uses the weight as it is.  No reference
+        counterpart."""
+        if on and self.weight.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"fp8 products need a bfloat16 or float32 weight (got {self.weight.dtype})")
+        self.fp8_products = bool(on)
+        return self
+
     def set_l2_manager(self, l2_manager):
         self._l2_manager = l2_manager
 
@@ -148,6 +162,11 @@ class FusedLinear(nn.Module):
             return F.linear(x, self.weight, self.bias)
         self._ensure_state()
         cfg = self._config
+        if self.fp8_products:
+            if not x.is_cuda or x.dtype != torch.bfloat16:
+                raise ValueError(f"fp8 products take bfloat16 CUDA activations (got {x.dtype} on {x.device})")
+            return FusedLinearFunction.apply(x, self.weight, self.bias, self._state, cfg, self._is_accumulating, self._l2_manager,
+                                             self.use_fused_backward, self._update_group, True)
         if (cfg is not None and not self._is_accumulating and self.use_fused_backward and x.is_cuda
                 and x.dtype == torch.bfloat16 and self._state._pending_grad is None):
             nat = native.module()
@@ -323,6 +342,12 @@ class FusedOptimizerManager:
             for m in members:
                 m._update_group = g
             self._update_groups.append(g)
+        return self
+
+    def use_fp8_products(self, on: bool = True, modules=None):
+        """``FusedLinear.use_fp8_products`` on every plain ``FusedLinear`` of the model, or on ``modules``."""
+        for m in (modules if modules is not None else [m for m in self._fused_modules if type(m) is FusedLinear]):
+            m.use_fp8_products(on)
         return self
 
     def flush_updates(self):

@@ -207,6 +207,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self._device_step = max((st["step"] for st in self.state.values() if st), default=0)
         return self
 
+    @property
+    def reads_device_hyper(self) -> bool:
+        return self._device_hyper is not None
+
     def _hyper_block(self, index, device):
         hd = self._device_hyper.get((index, device))
         if hd is None:

@@ -232,6 +232,11 @@ class FusedRMSNormLinear(FusedLinear):
     def _gamma(self):
         return self._gamma_ref[0]
 
+    def use_fp8_products(self, on: bool = True):
+        if on:
+            raise ValueError("fp8 products are not available on FusedRMSNormLinear: its backward recomputes the activation")
+        return self
+
     def forward(self, hidden_states):
         if not self.training:
             return F.linear(rmsnorm_forward(hidden_states, self._gamma, self._eps), self.weight, self.bias)
