@@ -248,6 +248,15 @@ struct Vec<DT_BF16> {
   static __device__ __forceinline__ float one(const uint8_t* p) {
     return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16);
   }
+  // the vector's first element, which it loses
+  static __device__ __forceinline__ float pop(uint4& q) {
+    const float x = __uint_as_float(q.x << 16);
+    q.x = __funnelshift_r(q.x, q.y, 16);
+    q.y = __funnelshift_r(q.y, q.z, 16);
+    q.z = __funnelshift_r(q.z, q.w, 16);
+    q.w >>= 16;
+    return x;
+  }
 };
 template <>
 struct Vec<DT_F32> {
@@ -264,6 +273,11 @@ struct Vec<DT_F32> {
     return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
   }
   static __device__ __forceinline__ float one(const uint8_t* p) { return *reinterpret_cast<const float*>(p); }
+  static __device__ __forceinline__ float pop(uint4& q) {
+    const float x = __uint_as_float(q.x);
+    q = make_uint4(q.y, q.z, q.w, 0);
+    return x;
+  }
 };
 
 __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
@@ -282,14 +296,15 @@ struct Shared {
   Acc cta_acc[MAX_CLUSTER];              // written by the cluster's CTAs into the first one's copy
 };
 struct alignas(16) TopShared {
-  u64 cand[CAP];
+  u64 cand[CAP];                         // keys
+  uint32_t col[CAP];                     // columns of candidates that have no key yet
   u64 best[32];                          // ranked, descending
   u64 cta_keys[MAX_CLUSTER * 32];        // as cta_acc
   float warp_bound[WARPS];
   int count;
 };
 
-// the best 32 of cand[0 .. n) in order of rank, into best[] (0 where there are fewer); all threads call it
+// The best 32 of cand[0 .. n) in order of rank, into best[] (0 where there are fewer); all threads call it.
 __device__ __forceinline__ void rank_keys(const u64* cand, int n, u64* best) {
   if (threadIdx.x < 32) best[threadIdx.x] = 0;
   __syncthreads();
@@ -327,6 +342,39 @@ __device__ __forceinline__ void write_row(const Params& p, long long row, const 
     p.top_ids[row * p.top_k + lane] = list != 0 ? static_cast<long long>(key_index(list)) : lane;
     p.top_logprobs[row * p.top_k + lane] = ((list != 0 ? key_value(list) : NAN) * p.inv_t - a.m) - log_s;
   }
+}
+
+// a CTA's columns: vectors [v_begin, v_end) from vbase on, the first of them column `head`, and `ones` single ones, those in
+// front of `head` and those from `tail` on
+struct Columns {
+  const uint8_t* vbase;
+  const uint8_t* base;
+  int v_begin, v_end, head, tail, ones;
+  uint32_t first;
+};
+
+// the best 32 keys of this warp's share of the CTA's columns, sorted over its lanes
+template <int DT>
+__device__ __noinline__ u64 rescan(const Columns& c, int top_k) {
+  using V = Vec<DT>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 list = 0, floor_key = 0;
+  for (int v0 = c.v_begin + warp * 32; v0 < c.v_end; v0 += THREADS) {
+    const int v = v0 + lane;
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (v < c.v_end) q = load_stream(c.vbase + static_cast<long long>(v) * 16);
+#pragma unroll 1
+    for (int i = 0; i < V::N; ++i) {
+      const float x = V::pop(q);
+      warp_offer(list, floor_key, v < c.v_end ? make_key(x, c.first + c.head + v * V::N + i) : 0, top_k, lane);
+    }
+  }
+  if (warp == 0) {
+    const int col = lane < c.head ? lane : c.tail + (lane - c.head);
+    const bool live = lane < c.ones;
+    warp_offer(list, floor_key, live ? make_key(V::one(c.base + static_cast<long long>(live ? col : 0) * V::ES), c.first + col) : 0, top_k, lane);
+  }
+  return list;
 }
 
 template <int DT, bool TOP>
@@ -369,28 +417,19 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(const 
 
   constexpr int U = 4;
   float bound = -INFINITY;               // nothing below it can be among the best k
-  if constexpr (TOP) {
-    if (threadIdx.x == 0) top.count = 0;
-    __syncthreads();
+  // At most N - 1 single columns at either end: warp 0 of the first CTA, one per lane.
+  const int n_one = rank == 0 ? head + vocab - tail0 : 0;
+  if (TOP && threadIdx.x == 0) top.count = n_one;
+  if (warp == 0 && lane < n_one) {
+    const int col = lane < head ? lane : tail0 + (lane - head);
+    const float x[1] = {V::one(base + static_cast<long long>(col) * ES)};
+    if (x[0] > r.thr) rebase(r, x[0], lazy, c);
+    accumulate_raw<1>(r, x, c);
+    if constexpr (TOP) top.col[lane] = col;
   }
-  auto push = [&](float x, int col) {
-    const int at = atomicAdd(&top.count, 1);
-    if (at < CAP) top.cand[at] = make_key(x, static_cast<uint32_t>(p.vocab_start) + col);
-  };
-  // candidates -> the best 32 of them and a new bound; false if there were too many to keep
-  auto rank_down = [&]() {
-    __syncthreads();
-    const int n = top.count;
-    if (n > CAP) return false;
-    rank_keys(top.cand, n, top.best);
-    if (threadIdx.x < 32) top.cand[threadIdx.x] = top.best[threadIdx.x];
-    if (threadIdx.x == 0) top.count = 32;
-    const u64 kth = top.best[p.top_k - 1];
-    if (kth != 0) bound = key_value(kth);
-    __syncthreads();
-    return true;
-  };
-  bool kept = true;                      // every candidate is in top.cand
+  if constexpr (TOP) __syncthreads();
+  int keyed = 0;                         // candidates below this have their keys in top.cand
+  bool kept = true;                      // every candidate is in the list
 
   // vectors past the end are all masked
   auto load = [&](int v0, uint4 (&q)[U]) {
@@ -404,10 +443,12 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(const 
   };
   uint4 q[U], ahead[U];
   load(v_begin, ahead);
-  for (int v0 = v_begin, batch = 1, next_rank = 1; v0 < v_end; v0 += U * THREADS, ++batch) {
+  // (once at least: the last batch ranks the candidates)
+  for (int v0 = v_begin, batch = 1, next_rank = 1; v0 < v_end || batch == 1; v0 += U * THREADS, ++batch) {
+    const bool last = v0 + U * THREADS >= v_end;
 #pragma unroll
     for (int u = 0; u < U; ++u) q[u] = ahead[u];
-    if (v0 + U * THREADS < v_end) load(v0 + U * THREADS, ahead);
+    if (!last) load(v0 + U * THREADS, ahead);
     float mx = V::max_of(q[0]);
 #pragma unroll
     for (int u = 1; u < U; ++u) mx = fmaxf(mx, V::max_of(q[u]));
@@ -436,7 +477,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(const 
       }
     }
     if constexpr (TOP) {
-      if (v0 == v_begin) {
+      if (batch == 1) {
         // the first bound, from the threads' maxima of this batch
         const int full = min(WARPS, (v_end - v_begin) / 32);         // warps whose first vectors are all live
         if (full > 0 && warp < full) {
@@ -457,33 +498,52 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(const 
         }
       }
       if (kept && mx >= bound) {
+        // one place in the list per thread for all of its candidates
+        uint32_t mask = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int v = v0 + u * THREADS + threadIdx.x;
-          if (v < v_end && V::max_of(q[u]) >= bound) {
-            float x[N];
-            V::unpack(q[u], x);
+          float x[N];
+          V::unpack(q[u], x);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-              if (x[i] >= bound) push(x[i], head + v * N + i);
+          for (int i = 0; i < N; ++i) mask |= x[i] >= bound ? 1u << (u * N + i) : 0u;
+          if (v0 + u * THREADS + static_cast<int>(threadIdx.x) >= v_end) mask &= (1u << (u * N)) - 1u;
+        }
+        int at = atomicAdd(&top.count, __popc(mask));
+#pragma unroll 1
+        for (; mask != 0; mask &= mask - 1, ++at) {
+          const int e = __ffs(mask) - 1;
+          if (at < CAP) top.col[at] = head + (v0 + (e / N) * THREADS + static_cast<int>(threadIdx.x)) * N + e % N;
+        }
+      }
+      if (batch == next_rank || last) {
+        next_rank *= 4;
+        __syncthreads();
+        int n = top.count;
+        __syncthreads();
+        kept = n <= CAP;
+        if (kept || last) {
+          if (kept) {
+            for (int i = keyed + static_cast<int>(threadIdx.x); i < n; i += THREADS) {
+              const uint32_t col = top.col[i];
+              top.cand[i] = make_key(V::one(base + static_cast<long long>(col) * ES), static_cast<uint32_t>(p.vocab_start) + col);
+            }
+          } else {
+            // once more, each warp for itself
+            const Columns cols{vbase, base, v_begin, v_end, head, tail0, n_one, static_cast<uint32_t>(p.vocab_start)};
+            top.cand[warp * 32 + lane] = rescan<DT>(cols, p.top_k);
+            n = WARPS * 32;
+          }
+          rank_keys(top.cand, n, top.best);
+          if (!last) {
+            if (threadIdx.x < 32) top.cand[threadIdx.x] = top.best[threadIdx.x];
+            if (threadIdx.x == 0) top.count = 32;
+            keyed = 32;
+            const u64 kth = top.best[p.top_k - 1];
+            if (kth != 0) bound = key_value(kth);
+            __syncthreads();
           }
         }
       }
-      if (batch == next_rank && v0 + U * THREADS < v_end) {
-        next_rank *= 4;
-        kept = kept && rank_down();
-      }
-    }
-  }
-  // at most N - 1 single columns at either end: warp 0 of the first CTA, one per lane
-  if (rank == 0 && warp == 0) {
-    const int n_one = head + vocab - tail0;
-    const int col = lane < head ? lane : tail0 + (lane - head);
-    if (lane < n_one) {
-      const float x[1] = {V::one(base + static_cast<long long>(col) * ES)};
-      if (x[0] > r.thr) rebase(r, x[0], lazy, c);
-      accumulate_raw<1>(r, x, c);
-      if (TOP && x[0] >= bound) push(x[0], col);
     }
   }
 
@@ -493,32 +553,6 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(const 
   if (lane == 0) sh.warp_acc[warp] = a;
   __syncthreads();
   if (warp == 0) a = warp_join(lane < WARPS ? sh.warp_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
-  if constexpr (TOP) {
-    int n = top.count;
-    __syncthreads();
-    if (n > CAP) {
-      // once more, each warp for itself
-      u64 list = 0, floor_key = 0;
-      for (int v0 = v_begin + warp * 32; v0 < v_end; v0 += THREADS) {
-        const int v = v0 + lane;
-        float x[N];
-        if (v < v_end) V::unpack(load_stream(vbase + static_cast<long long>(v) * 16), x);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          warp_offer(list, floor_key, v < v_end ? make_key(x[i], static_cast<uint32_t>(p.vocab_start) + head + v * N + i) : 0, p.top_k, lane);
-      }
-      if (rank == 0 && warp == 0) {
-        const int col = lane < head ? lane : tail0 + (lane - head);
-        warp_offer(list, floor_key,
-                   lane < head + vocab - tail0 ? make_key(V::one(base + static_cast<long long>(col) * ES), static_cast<uint32_t>(p.vocab_start) + col) : 0,
-                   p.top_k, lane);
-      }
-      top.cand[warp * 32 + lane] = list;
-      n = WARPS * 32;
-      __syncthreads();
-    }
-    rank_keys(top.cand, n, top.best);
-  }
   if (cs > 1) {
     __syncwarp();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");       // the first CTA has started
