@@ -6,15 +6,11 @@
 //   Y[m, n] = sum over kb of sx[m, kb] sw[n / 128, kb] * sum over the block's k of xq[m, k] wq[n, k]
 //
 // The inner sums are tensor-core products of 128 terms; the outer sum is held in fp32 registers.
-#include <cooperative_groups.h>
-
 #include <algorithm>
 #include <atomic>
 
 #include "forge_host.h"
 #include "forge_ptx.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace forge {
 namespace fp8 {
@@ -277,8 +273,12 @@ struct Cfg {
   static constexpr int B_BYTES = NT * BK;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   // up to 64 tokens two CTAs share an SM (112 KB each); 128 take an SM's tensor memory alone
-  static constexpr int STAGES = NT == 128 ? 6 : (NT == 64 ? 4 : 5);
-  static constexpr int SMEM = 1024 + STAGES * STAGE;      // + alignment slack; control words are static
+  static constexpr int STAGES = NT == 128 ? 6 : (NT == 64 ? 3 : (NT == 32 ? 4 : 5));
+  // what the cluster's CTAs send for this CTA's tokens: at most NT + split - 1 rows of 128 sums.  With 128 tokens there is
+  // no room for it beside the stages: it takes their place, once all CTAs of the cluster are done with theirs.
+  static constexpr bool SHARED_RECV = NT == 128;
+  static constexpr int RECV = (NT + 8) * 128 * 4;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + (SHARED_RECV ? 0 : RECV);      // + alignment slack; control words are static
   static constexpr int TMEM_COLS = ACC_BUFS * NT;
   static constexpr int MIN_CTAS = NT == 128 ? 1 : 2;
 };
@@ -289,6 +289,13 @@ __device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t* r) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr)
                : "memory");
+}
+
+// the first barrier phase of a cluster: everybody has started
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
 // instruction descriptor of kind::f8f6f4, e4m3 x e4m3 -> f32, both operands K-major
@@ -314,9 +321,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return u;
 }
 
+constexpr int MAX_STAGES = 6;
 struct Ctrl {
-  uint64_t full[8];
-  uint64_t empty[8];
+  uint64_t full[MAX_STAGES];
+  uint64_t empty[MAX_STAGES];
   uint64_t acc_full[ACC_BUFS];
   uint64_t acc_empty[ACC_BUFS];
   uint64_t sc_full[SC_SLOTS];
@@ -361,6 +369,7 @@ template <int NT>
 __global__ void __launch_bounds__(THREADS, Cfg<NT>::MIN_CTAS)
 fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params p) {
   using C = Cfg<NT>;
+  static_assert(C::STAGES <= MAX_STAGES, "one barrier pair per stage");
   __shared__ Ctrl ctrl;
   __shared__ __align__(16) float sc[SC_SLOTS][NT];
   extern __shared__ uint8_t smem_raw[];
@@ -373,6 +382,14 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   const int m0 = (tile % p.tiles_m) * NT, n0 = (tile / p.tiles_m) * 128;
   const int per = (p.KB + p.split - 1) / p.split;
   const int kb0 = min(p.KB, rank * per), kb1 = min(p.KB, kb0 + per);
+  // where the sums of this CTA's tokens are: its own, if K is not cut, lie at the start of the stages (see below)
+  float* recv = reinterpret_cast<float*>(p.split == 1 ? data : data + (C::SHARED_RECV ? NT * 512 : C::STAGES * C::STAGE));
+  static_assert(!C::SHARED_RECV || NT * 512 + C::RECV <= C::STAGES * C::STAGE, "the sums fit where the stages were");
+  // the tile's tokens, and how many of them each CTA of the cluster writes
+  const int tokens = min(NT, p.M - m0), share = (tokens + p.split - 1) / p.split;
+  // (waited for before anything is sent to another CTA: it has started)
+  if (p.split > 1 && !C::SHARED_RECV) cluster_arrive_relaxed();
+  const uint64_t pol_w = p.tiles_m > 1 ? policy_evict_normal() : policy_evict_first();
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; ++i) { mbar_init(&ctrl.full[i], 1); mbar_init(&ctrl.empty[i], 1); }
@@ -380,14 +397,17 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     for (int i = 0; i < SC_SLOTS; ++i) { mbar_init(&ctrl.sc_full[i], 2); mbar_init(&ctrl.sc_empty[i], 8); }
     ctrl.abort_word = 0;
     mbar_fence_init();
+    fence_proxy_async_smem();
+    // the weight's first stages are on their way before the rest of the CTA is set up, and (early) before the tokens'
+    // codes are known to be there
+    for (int i = 0; i < C::STAGES && kb0 + i < kb1; ++i) {
+      mbar_expect_tx(&ctrl.full[i], C::STAGE);
+      tma_load_2d(data + i * C::STAGE, &tm_w, &ctrl.full[i], (kb0 + i) * BK, n0, pol_w);
+    }
   }
   if (warp == 1) {
     tmem_alloc(&ctrl.tmem_base, C::TMEM_COLS);
     tmem_relinquish();
-  }
-  if (warp == 0 && lane == 0) {
-    prefetch_tmap(&tm_w);
-    prefetch_tmap(&tm_x);
   }
   tc_fence_before();
   __syncthreads();
@@ -396,25 +416,18 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint64_t pol_w = p.tiles_m > 1 ? policy_evict_normal() : policy_evict_first();
       const uint64_t pol_x = policy_evict_last();
-      // (early: the weight's first stages are asked for before the tokens' codes are known to be there)
-      auto second_operand = [&]() {
-        wait_for_previous();
-        for (int i = 0; i < min(C::STAGES, kb1 - kb0); ++i)
-          tma_load_2d(data + i * C::STAGE + A_BYTES, &tm_x, &ctrl.full[i], (kb0 + i) * BK, m0, pol_x);
-      };
-      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+      if (p.early) wait_for_previous();
+      for (int i = 0; i < C::STAGES && kb0 + i < kb1; ++i)
+        tma_load_2d(data + i * C::STAGE + A_BYTES, &tm_x, &ctrl.full[i], (kb0 + i) * BK, m0, pol_x);
+      for (int kb = kb0 + C::STAGES, it = C::STAGES; kb < kb1; ++kb, ++it) {
         const int s = it % C::STAGES;
-        if (p.early && it == C::STAGES) second_operand();
         if (!mbar_wait(&ctrl.empty[s], ((it / C::STAGES) & 1) ^ 1, abort_word, ERR_OP_EMPTY)) break;
         uint8_t* a = data + s * C::STAGE;
         mbar_expect_tx(&ctrl.full[s], C::STAGE);
         tma_load_2d(a, &tm_w, &ctrl.full[s], kb * BK, n0, pol_w);
-        if (p.early && it < C::STAGES) continue;
         tma_load_2d(a + A_BYTES, &tm_x, &ctrl.full[s], kb * BK, m0, pol_x);
       }
-      if (p.early && kb1 - kb0 <= C::STAGES) second_operand();
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -479,8 +492,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
         mbar_arrive(&ctrl.sc_empty[slot]);
       }
     }
-    // Every product has completed (the last accumulator was signalled after all of them), so the operand
-    // stages are free: the part goes there as [token][weight row].
+    // Every product has completed (the last accumulator was signalled after all of them), so this CTA's operand stages are
+    // free: its sums go there as [token][weight row].
     float* part = reinterpret_cast<float*>(data);
     const int r = quarter * 32 + lane;
 #pragma unroll
@@ -496,40 +509,44 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     while (clock64() - t0 < 400000) __nanosleep(1000);
     if (threadIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, 0, *abort_word);
   }
-  cg::cluster_group cluster = cg::this_cluster();
-  if (p.split > 1) cluster.sync();
-  {
-    // this CTA's share of the tile's tokens: eight weight rows per lane, sixteen lanes per token
-    const int tokens = min(NT, p.M - m0);
-    const int share = (tokens + p.split - 1) / p.split;
-    const int j1 = min(tokens, (rank + 1) * share);
-    const int r8 = (threadIdx.x & 15) * 8;
-    for (int j = rank * share + (threadIdx.x >> 4); j < j1; j += THREADS / 16) {
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-      for (int q = 0; q < p.split; ++q) {
-        const float* part = reinterpret_cast<const float*>(p.split > 1 ? cluster.map_shared_rank(data, q) : data);
-        const float4 a = *reinterpret_cast<const float4*>(part + j * 128 + r8);
-        const float4 c = *reinterpret_cast<const float4*>(part + j * 128 + r8 + 4);
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-        v[4] += c.x; v[5] += c.y; v[6] += c.z; v[7] += c.w;
-      }
-      __nv_bfloat16* dst = p.y + static_cast<long long>(m0 + j) * p.ld_y + n0 + r8;
-      if (failed) continue;
-      if (p.wide && n0 + r8 + 8 <= p.N) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (n0 + r8 + k < p.N) dst[k] = __float2bfloat16_rn(v[k]);
-      }
+  __syncwarp();
+  if (p.split > 1) {
+    if (C::SHARED_RECV) cluster_arrive_relaxed();       // (now it means: this CTA no longer needs its stages)
+    cluster_wait();
+    // each token's sums go to the CTA that adds them up and writes them, row [this rank][token] there
+    const float* part = reinterpret_cast<const float*>(data);
+    for (int j = warp; j < tokens; j += THREADS / 32) {
+      const float4 v = *reinterpret_cast<const float4*>(part + j * 128 + lane * 4);
+      st_cluster(map_to_cta(smem_u32(recv + (rank * share + j % share) * 128 + lane * 4), j / share), v);
     }
+    __syncwarp();
+    cluster_sync_all();                                  // all sums have arrived; nothing is sent after this
   }
-  if (p.split > 1) cluster.sync();          // a part stays until every CTA of the cluster has read it
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+  // this CTA's tokens: eight weight rows per lane, sixteen lanes per token, the parts added in the order of the ranks
+  const int j1 = min(tokens - rank * share, share);
+  const int r8 = (threadIdx.x & 15) * 8;
+  for (int j = threadIdx.x >> 4; j < j1 && !failed; j += THREADS / 16) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    for (int q = 0; q < p.split; ++q) {
+      const float4 a = *reinterpret_cast<const float4*>(recv + (q * share + j) * 128 + r8);
+      const float4 c = *reinterpret_cast<const float4*>(recv + (q * share + j) * 128 + r8 + 4);
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += c.x; v[5] += c.y; v[6] += c.z; v[7] += c.w;
+    }
+    __nv_bfloat16* dst = p.y + static_cast<long long>(m0 + rank * share + j) * p.ld_y + n0 + r8;
+    if (p.wide && n0 + r8 + 8 <= p.N) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (n0 + r8 + k < p.N) dst[k] = __float2bfloat16_rn(v[k]);
+    }
   }
 }
 

@@ -792,13 +792,15 @@ extern "C" int forge_logprobs_forward(const ForgeLogprobsArgs* args, void* cuda_
   const DeviceInfo* di = current_device_info();
   if (di == nullptr) return FORGE_ERR_CUDA;
   if (di->cc_major != 10) return fail(FORGE_ERR_DEVICE, "device %d is sm_%d%d, not sm_100", di->device, di->cc_major, di->cc_minor);
-  // A row is cut over a cluster while two CTAs per SM hold all of them and each still has two vectors per thread
-  // to load: 64 rows of 128256 bf16 logits take 14.6 / 9.7 / 7.7 / 10.2 us over 1 / 2 / 4 / 8 CTAs a row, 4096 fp32
-  // logits 4.7 / 5.9 us over 1 / 2.  The first CTA ranks the others' k keys each: with k = 20, 8 CTAs a row beat 16
-  // (14.6 against 18.5 us for 16 rows).
+  // A row is cut over a cluster while all CTAs are resident at once and each still has two vectors per thread to load:
+  // 64 rows of 128256 bf16 logits take 14.2 / 9.6 / 7.6 / 10.3 us over 1 / 2 / 4 / 8 CTAs a row, 200 rows 17.5 / 15.3 / 17.8
+  // over 1 / 2 / 4, 4096 fp32 logits 4.7 / 5.9 us over 1 / 2.  (Clusters of eight and sixteen fill the GPU less well: two CTAs
+  // per SM instead of 2.7.)  The first CTA ranks the others' k keys each: with k = 20, 8 CTAs a row beat 16 (14.6 against
+  // 18.5 us for 16 rows).
   const long long vecs = a.vocab * es / 16;
+  auto resident = [&](int n) { return a.rows * n * 10 <= (n <= 4 ? 27ll : 20ll) * di->sm_count; };
   int cs = 1;
-  while (cs < loss::MAX_CLUSTER && a.rows * cs * 2 <= 2ll * di->sm_count && vecs > 4ll * cs * loss::THREADS && cs * 2 * a.top_k <= 192) cs *= 2;
+  while (cs < loss::MAX_CLUSTER && resident(cs * 2) && vecs > 4ll * cs * loss::THREADS && cs * 2 * a.top_k <= 192) cs *= 2;
   const loss::Params p = loss::make_params(a);
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   if (a.dtype == FORGE_DT_BF16)

@@ -89,7 +89,7 @@ def check_product(xq, xs, wq, ws, y):
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {((y.double() - want).abs() / tol.clamp(min=1e-300)).max():.2f}x"
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 1, 1), (1, 1030, 4096), (2, 130, 300), (16, 256, 512), (17, 129, 1000), (33, 640, 144),
+@pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 1, 1), (1, 1030, 4096), (1, 20000, 700), (2, 5000, 1040), (2, 130, 300), (3, 777, 5000), (4, 6000, 514), (4, 129, 16), (5, 20001, 1168), (8, 4100, 2064), (7, 33, 130), (16, 256, 512), (17, 129, 1000), (33, 640, 144),
                                    (64, 1024, 2048), (65, 257, 384), (128, 128, 128), (129, 300, 520), (200, 1024, 7168), (500, 2000, 640),
                                    (512, 4096, 1024), (700, 515, 260), (1100, 3000, 900), (5, 14336, 4096), (2048, 1024, 256)])
 def test_product_against_64_bits(m, n, k):
