@@ -62,23 +62,6 @@ __device__ __forceinline__ int find_tensor(const int* first, int count, int c) {
 }
 
 template <int DT>
-__device__ __forceinline__ void load8(const void* base, long long i, float (&x)[8]) {
-  if constexpr (DT == DT_F32) {
-    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
-    const float4 a = q[0], b = q[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[2 * k] = __uint_as_float(u[k] << 16);
-      x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-    }
-  }
-}
-template <int DT>
 __device__ __forceinline__ void store8(void* base, long long i, const float (&x)[8]) {
   if constexpr (DT == DT_F32) {
     float4* q = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
@@ -87,19 +70,19 @@ __device__ __forceinline__ void store8(void* base, long long i, const float (&x)
   } else {
     uint32_t u[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = float_to_bf16_bits(x[2 * k]) | (float_to_bf16_bits(x[2 * k + 1]) << 16);
+    for (int k = 0; k < 4; ++k) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[k]) : "f"(x[2 * k + 1]), "f"(x[2 * k]));
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + i) = make_uint4(u[0], u[1], u[2], u[3]);
   }
-}
-template <int DT>
-__device__ __forceinline__ float load1(const void* base, long long i) {
-  if constexpr (DT == DT_F32) return static_cast<const float*>(base)[i];
-  else return bf16_bits_to_float(static_cast<const uint16_t*>(base)[i]);
 }
 template <int DT>
 __device__ __forceinline__ void store1(void* base, long long i, float x) {
   if constexpr (DT == DT_F32) static_cast<float*>(base)[i] = x;
   else static_cast<uint16_t*>(base)[i] = static_cast<uint16_t>(float_to_bf16_bits(x));
+}
+
+__device__ __forceinline__ float absmax8(const float (&x)[8]) {
+  const float a = fmax3(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])), b = fmax3(fabsf(x[3]), fabsf(x[4]), fabsf(x[5]));
+  return fmax3(fmaxf(a, b), fabsf(x[6]), fabsf(x[7]));
 }
 
 __device__ __forceinline__ bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -250,12 +233,18 @@ __global__ void __launch_bounds__(THREADS) multi_adamw_kernel(const __grid_const
     }
     uint32_t mo[2], vo[2];
     if constexpr (QUANT) {
-      float am = 0.0f, av = 0.0f;
-#pragma unroll
-      for (int k = 0; k < EPT; ++k) {
+      float am, av;
+      if (live == EPT) {
+        am = absmax8(m);
+        av = absmax8(v);
+      } else {
         // elements past the end of the tensor take no part in the last block's absmax
-        am = fmaxf(am, k < live ? fabsf(m[k]) : 0.0f);
-        av = fmaxf(av, k < live ? fabsf(v[k]) : 0.0f);
+        am = av = 0.0f;
+#pragma unroll
+        for (int k = 0; k < EPT; ++k) {
+          am = fmaxf(am, k < live ? fabsf(m[k]) : 0.0f);
+          av = fmaxf(av, k < live ? fabsf(v[k]) : 0.0f);
+        }
       }
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) {
@@ -351,21 +340,25 @@ __global__ void __launch_bounds__(THREADS) multi_norm_kernel(const __grid_consta
   const long long begin = static_cast<long long>(chunk - p.first_chunk[ti]) * p.passes * PASS;
   const bool wide = aligned(it.g, 16);
   double sum = 0.0;
-#pragma unroll 4
-  for (int pass = 0; pass < p.passes; ++pass) {
+  constexpr int AT_ONCE = 4;                    // passes whose elements are on their way together
+  for (int pass = 0; pass < p.passes; pass += AT_ONCE) {
     const long long i0 = begin + static_cast<long long>(pass) * PASS + threadIdx.x * EPT;
-    if (i0 >= it.n) break;
-    float x[EPT];
-    if (wide && i0 + EPT <= it.n) {
-      load8<DT>(it.g, i0, x);
-    } else {
+    Raw8<DT> raw[AT_ONCE];
 #pragma unroll
-      for (int k = 0; k < EPT; ++k) x[k] = i0 + k < it.n ? load1<DT>(it.g, i0 + k) : 0.0f;
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const long long i = i0 + u * PASS;
+      const int live = pass + u < p.passes ? live_of(it.n, i) : 0;
+      if (wide && live == EPT) raw[u].load(it.g, i);
+      else raw[u].load_some(it.g, i, live);
     }
-    float s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < EPT; ++k) s = __fmaf_rn(x[k], x[k], s);
-    sum += static_cast<double>(s);
+    for (int u = 0; u < AT_ONCE; ++u) {
+      float x[EPT], s = 0.0f;
+      raw[u].get(x);
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) s = __fmaf_rn(x[k], x[k], s);
+      sum += static_cast<double>(s);
+    }
   }
   const double t = block_sum_d(sum, red);
   if (threadIdx.x == 0) p.partial[blockIdx.x] = t;

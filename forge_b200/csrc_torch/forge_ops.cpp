@@ -280,6 +280,10 @@ py::object multi_adamw(const py::object& params, const py::object& grads, const 
   a.hyper = ForgeHyper{lr, beta1, beta2, eps, weight_decay, 0.0, 0, static_cast<int32_t>(step)};
   a.hyper_device = reinterpret_cast<const void*>(hyper_device);
   check(forge_multi_adamw(&a, stream), "forge_multi_adamw");
+  // for autograd: a graph that has saved one of these tensors must not go on with other values
+  for (const auto* list : {&p, &m, &v})
+    for (const at::Tensor* t : *list)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return py::make_tuple(true, max_norm > 0 ? py::reinterpret_steal<py::object>(THPVariable_Wrap(out.select(0, 0))) : none);
 }
 

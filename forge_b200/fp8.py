@@ -125,7 +125,8 @@ def fp8_matmul(x_codes, x_scales, w_codes, w_scales) -> torch.Tensor:
 
 
 class Fp8Weight:
-    """Codes and scales of a weight (N, K) in 128 x 128 blocks and, for input gradients, of its transpose."""
+    """Codes and scales of a weight (N, K) in 128 x 128 blocks and, for input gradients, of its transpose.  A backward pass
+    reads the transposed codes as they are then: call ``update_`` after it."""
 
     __slots__ = ("codes", "scales", "codes_t", "scales_t")
 
@@ -191,7 +192,7 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Weight, bias: torch.Tensor | None = N
     _require_cuda(x, bias)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"fp8_linear takes bfloat16 activations (got {x.dtype})")
-    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] == 0:
         raise ValueError(f"x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
     if not torch.is_grad_enabled() or not (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _forward(x, bias, weight)

@@ -162,7 +162,8 @@ class _TokenLogprobs(torch.autograd.Function):
             top, ids = top.view(*lead, top_k), ids.view(*lead, top_k)
             ctx.mark_non_differentiable(top, ids)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, t, lse, ent)
+        # the logits themselves where they are rows already, so that autograd notices if they are changed
+        ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, t, lse, ent)
         ctx.shape = logits.shape
         ctx.settings = (temperature, ignore_index, vocab_start, vocab_total)
         return lp, ent, top, ids
@@ -171,6 +172,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_ent, _g_top, _g_ids):
         x, t, lse, ent = ctx.saved_tensors
+        x = _rows(x)
         none = (None,) * 7
         if g_lp is None and g_ent is None:
             return (None, *none)

@@ -156,6 +156,8 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None
     with torch.cuda.device(dev):
         rc = _lib.load().forge_multi_adamw(ctypes.byref(a), _lib.current_stream_ptr(dev))
     _lib.check(rc, "forge_multi_adamw")
+    # (for autograd: a graph that has saved one of these tensors must not go on with other values)
+    torch.autograd.graph.increment_version([t for t in (*params, *exp_avgs, *exp_avg_sqs) if not t.is_inference()])
     return norm
 
 
@@ -172,6 +174,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                  state_mode: str = "f32", max_grad_norm: float | None = None):
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError(f"max_grad_norm must be positive (got {max_grad_norm})")
+        if not lr >= 0 or not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"lr={lr}, betas={betas}, eps={eps}, weight_decay={weight_decay}: out of range")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_mode=state_mode))
         for group in self.param_groups:
             self._check_group(group)
@@ -229,6 +233,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise ValueError("pre_step() belongs to enable_device_hyper()")
         self._device_step += 1
         for index, group in enumerate(self.param_groups):
+            for p in group["params"]:              # (a replayed step() does not come by here)
+                if self.state.get(p):
+                    self.state[p]["step"] = self._device_step
             for dev in {p.device for p in group["params"]}:
                 hd = self._device_hyper.get((index, dev))
                 if hd is None:

@@ -204,6 +204,23 @@ def test_gradient_against_differences():
             assert abs(float((f(base + d) - f(base - d)) / (2 * h)) - float(dx[r, j])) < 1e-5
 
 
+def test_second_derivatives_are_refused_and_changed_logits_noticed():
+    x, t = make(3, 50, torch.float32, seed=31)
+    x = x.requires_grad_(True)
+    for view in (x, x[:, 1:]):                         # the direct call; rows of a wider pitch
+        out = token_logprobs(view, t.clamp(max=48))
+        (dx,) = torch.autograd.grad(out.logprobs.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(dx.sum(), x)
+    y = x.detach().clone().requires_grad_(True)
+    z = y * 1.0
+    out = token_logprobs(z, t)
+    z.data.add_(0)
+    z.detach().add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.logprobs.sum().backward()
+
+
 def test_reproducible_streams_and_graph():
     x, t = make(33, 50001, torch.bfloat16, seed=14)
     x = x.requires_grad_(True)

@@ -320,6 +320,29 @@ def test_optimizer_in_a_graph():
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("strided", [False, True])
+def test_autograd_sees_the_update(strided):
+    """A graph that has saved a parameter refuses to go on once the step has changed it (both ways into the library)."""
+    w = torch.nn.Parameter(torch.ones(8, 8, device=DEV))
+    x = torch.ones(3, 8, device=DEV, requires_grad=True)
+    y = (x @ w).sum()
+    g = torch.ones(8, 16, device=DEV)[:, ::2] if strided else torch.ones(8, 8, device=DEV)
+    multi_tensor_adamw([w.detach()], [g], [torch.zeros(8, 8, device=DEV)], [torch.zeros(8, 8, device=DEV)])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_replayed_steps_are_counted_in_checkpoints():
+    p = torch.nn.Parameter(torch.ones(8, device=DEV))
+    p.grad = torch.ones(8, device=DEV)
+    opt = MultiTensorAdamW([p]).enable_device_hyper()
+    opt.pre_step()
+    opt.step()
+    for _ in range(3):
+        opt.pre_step()                                # (replays of a captured step() in between)
+    assert opt.state_dict()["state"][0]["step"] == 4
+
+
 def test_refusals():
     p, g = torch.zeros(8, 8, device=DEV), torch.zeros(8, 8, device=DEV)
     m, v = torch.zeros(8, 8, device=DEV), torch.zeros(8, 8, device=DEV)
@@ -342,5 +365,8 @@ def test_refusals():
         MultiTensorAdamW([torch.nn.Parameter(p)], state_mode="fp4")
     with pytest.raises(ValueError):
         MultiTensorAdamW([torch.nn.Parameter(p)], max_grad_norm=-1.0)
+    for kw in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(lr=math.nan)):
+        with pytest.raises(ValueError):
+            MultiTensorAdamW([torch.nn.Parameter(p)], **kw)
     with pytest.raises(ValueError):
         MultiTensorAdamW([torch.nn.Parameter(p)]).pre_step()
