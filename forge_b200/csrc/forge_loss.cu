@@ -378,7 +378,10 @@ __device__ __noinline__ u64 rescan(const Columns& c, int top_k) {
 }
 
 template <int DT, bool TOP>
-__global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(const Params p, const int cs) {
+// CTAs per SM: four of 64 registers (511 rows of 151936 fp32 logits take 69 us with three, 52 with four: one wave instead
+// of two).  With the top k three: the two registers that spill otherwise cost more than the fourth CTA brings (300 rows of
+// 128256 bf16 logits, k = 5: 32.5 against 37.4 us; 511 of 151936 fp32, k = 20, the other way: 80 against 73).
+__global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Params p, const int cs) {
   using V = Vec<DT>;
   constexpr int N = V::N, ES = V::ES;
   __shared__ Shared sh;
@@ -792,13 +795,13 @@ extern "C" int forge_logprobs_forward(const ForgeLogprobsArgs* args, void* cuda_
   const DeviceInfo* di = current_device_info();
   if (di == nullptr) return FORGE_ERR_CUDA;
   if (di->cc_major != 10) return fail(FORGE_ERR_DEVICE, "device %d is sm_%d%d, not sm_100", di->device, di->cc_major, di->cc_minor);
-  // A row is cut over a cluster while all CTAs are resident at once and each still has two vectors per thread to load:
-  // 64 rows of 128256 bf16 logits take 14.2 / 9.6 / 7.6 / 10.3 us over 1 / 2 / 4 / 8 CTAs a row, 200 rows 17.5 / 15.3 / 17.8
-  // over 1 / 2 / 4, 4096 fp32 logits 4.7 / 5.9 us over 1 / 2.  (Clusters of eight and sixteen fill the GPU less well: two CTAs
-  // per SM instead of 2.7.)  The first CTA ranks the others' k keys each: with k = 20, 8 CTAs a row beat 16 (14.6 against
-  // 18.5 us for 16 rows).
+  // A row is cut over a cluster while all CTAs are resident at once (nine tenths of the places that the kernel's launch
+  // bounds leave, two CTAs per SM for clusters of eight and sixteen, which fill the GPU less well) and each still has four
+  // vectors per thread to load: 64 rows of 128256 bf16 logits take 14.2 / 9.6 / 7.6 / 10.3 us over 1 / 2 / 4 / 8 CTAs a
+  // row, 100 rows of 151936 fp32 logits 18.3 / 14.3 over 2 / 4, 4096 fp32 logits 4.7 / 5.9 over 1 / 2.  The first CTA
+  // ranks the others' k keys each: with k = 20, 8 CTAs a row beat 16 (14.6 against 18.5 us for 16 rows).
   const long long vecs = a.vocab * es / 16;
-  auto resident = [&](int n) { return a.rows * n * 10 <= (n <= 4 ? 27ll : 20ll) * di->sm_count; };
+  auto resident = [&](int n) { return a.rows * n * 10 <= (n > 4 ? 20ll : a.top_k > 0 ? 27ll : 36ll) * di->sm_count; };
   int cs = 1;
   while (cs < loss::MAX_CLUSTER && resident(cs * 2) && vecs > 4ll * cs * loss::THREADS && cs * 2 * a.top_k <= 192) cs *= 2;
   const loss::Params p = loss::make_params(a);
