@@ -377,10 +377,10 @@ __device__ __noinline__ u64 rescan(const Columns& c, int top_k) {
   return list;
 }
 
-template <int DT, bool TOP>
 // CTAs per SM: four of 64 registers (511 rows of 151936 fp32 logits take 69 us with three, 52 with four: one wave instead
 // of two).  With the top k three: the two registers that spill otherwise cost more than the fourth CTA brings (300 rows of
 // 128256 bf16 logits, k = 5: 32.5 against 37.4 us; 511 of 151936 fp32, k = 20, the other way: 80 against 73).
+template <int DT, bool TOP>
 __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Params p, const int cs) {
   using V = Vec<DT>;
   constexpr int N = V::N, ES = V::ES;
@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const B
   auto one = [&](float x) {
     const float y = __fmaf_rn(x, c, nl);
     const float pr = exp2_approx(y);
-    if constexpr (ENT) return pr * __fmaf_rn(b, max_nan(y, -3.0e38f), a);
+    // (below -127 the probability is 0, and its logarithm must stay finite whatever b is)
+    if constexpr (ENT) return pr * __fmaf_rn(b, max_nan(y, -127.0f), a);
     else return pr * a;
   };
   const int mis = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / ES;

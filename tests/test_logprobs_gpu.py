@@ -184,6 +184,26 @@ def test_one_gradient_only_and_empty():
     assert y.grad.shape == (0, 700)
 
 
+@pytest.mark.parametrize("mask", ["inf", "lowest"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_entropy_gradient_at_masked_logits(dtype, mask):
+    """p log p is 0 at a masked logit, whatever its factor."""
+    x, t = make(5, 2003, dtype, masked=0.4, seed=41)
+    low = x if mask == "inf" else torch.where(x == -math.inf, torch.finfo(dtype).min, x.float()).to(dtype)
+    low = low.detach().requires_grad_(True)
+    out = token_logprobs(low, t, temperature=0.5)
+    gh = torch.tensor([-50.0, 3.0, 1e6, -1e30, 0.0], device=DEV)
+    (dx,) = torch.autograd.grad(out.entropy, low, gh)
+    hidden = x == -math.inf
+    assert (dx[hidden] == 0).all()
+    # the other columns: the gradient for -1, which test_masked_logits holds against the definition, times -gh
+    (unit,) = torch.autograd.grad(token_logprobs(low, t, temperature=0.5).entropy.sum(), low)
+    want = unit.double() * gh.double()[:, None]
+    # both are rounded to their type, from fp32 products of the same three factors (2^-22 each way)
+    tol = (torch.finfo(dtype).eps + 2.0 ** -20) * want.abs() + 2.0 ** -20 * gh.double().abs()[:, None] * 30
+    assert ((dx.double() - want).abs() <= tol)[~hidden].all()
+
+
 def test_gradient_against_differences():
     # exact in fp32: logits of a few bits, differences of the 64-bit function
     x, t = make(2, 37, torch.float32, seed=13, spread=1.0)
