@@ -680,6 +680,22 @@ __global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const B
   const long long v_begin = static_cast<long long>(blockIdx.x) * vec_per_cta;
   const long long v_end = v_begin + vec_per_cta < nv ? v_begin + vec_per_cta : nv;
   constexpr int U = BACK_VECS;
+  if (gl == 0.0f && gh == 0.0f) {
+    // neither result has a gradient (an ignored row, a padded one): zeros, whatever the row holds
+    auto zero = [&](long long col) { store_one<DT>(out + col * ES, 0.0f); };
+    for (long long v = v_begin + threadIdx.x; v < v_end; v += BACK_THREADS) {
+      if (wide) {
+        *reinterpret_cast<uint4*>(out + (head + v * N) * ES) = make_uint4(0, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) zero(head + v * N + i);
+      }
+    }
+    const long long tail0 = head + nv * N;
+    const int i = threadIdx.x;
+    if (blockIdx.x == 0 && i < head + (p.vocab - tail0)) zero(i < head ? i : tail0 + (i - head));
+    return;
+  }
   for (long long v = v_begin + threadIdx.x; v < v_end; v += U * BACK_THREADS) {
     uint4 q[U];
 #pragma unroll

@@ -353,7 +353,8 @@ int forge_logprobs_join(const ForgeLogprobsArgs* args, const float* stats, const
 /* grad[r, j] = (g_logprob[r] (1[j = t] - p_j) - g_entropy[r] p_j (log p_j + entropy[r])) / temperature, in the
  * logits' type, row pitch ld_grad.  args: as in the forward, with `lse` (and `entropy`, if g_entropy is given)
  * as it wrote them; the logits of a slice give the slice's columns of the gradient.  g_logprob, g_entropy:
- * (rows,) or NULL for zero. */
+ * (rows,) or NULL for zero.  A row for which both are zero (or the target is ignored and the second is) gets zeros,
+ * whatever its logits are. */
 int forge_logprobs_backward(const ForgeLogprobsArgs* args, const float* g_logprob, const float* g_entropy, void* grad,
                             int64_t ld_grad, void* cuda_stream);
 

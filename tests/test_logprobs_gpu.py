@@ -204,6 +204,21 @@ def test_large_entropy_gradient_at_masked_logits(dtype, mask):
     assert ((dx.double() - want).abs() <= tol)[~hidden].all()
 
 
+def test_rows_without_a_gradient_of_their_own():
+    """What a row holds is nobody's concern where neither of its results has a gradient: a padded row may be anything."""
+    for dtype in (torch.bfloat16, torch.float32):
+        for start in (0, 1):                              # rows that start off a 16-byte boundary, too
+            x, t = make(7, 3001, dtype, seed=42)
+            x[0], x[1], x[2, 7] = -math.inf, math.nan, math.inf
+            t[:4] = -100
+            view = x[:, start:].detach().requires_grad_(True)
+            out = token_logprobs(view, t.clamp(max=2999))
+            (dx,) = torch.autograd.grad(out.logprobs.sum(), view)
+            assert (dx[:4] == 0).all() and dx[4:].isfinite().all() and (dx[4:] != 0).any()
+            (dx,) = torch.autograd.grad(token_logprobs(view, t.clamp(max=2999)).logprobs[5:].sum(), view)
+            assert (dx[:5] == 0).all() and (dx[5:] != 0).any()
+
+
 def test_gradient_against_differences():
     # exact in fp32: logits of a few bits, differences of the 64-bit function
     x, t = make(2, 37, torch.float32, seed=13, spread=1.0)
