@@ -85,13 +85,14 @@ def _call(fn, device, *args):
         _lib.check(rc, fn)
 
 
-def _outputs(a, rows, top_k, device):
-    out = torch.empty(3, rows, dtype=torch.float32, device=device)
+def _outputs(a, lead, top_k, device):
+    # (tensors of their own and no views: what a user does in place to one result is not done to the saved ones)
+    out = [torch.empty(lead, dtype=torch.float32, device=device) for _ in range(3)]
     a.logprobs, a.entropy, a.lse = (t.data_ptr() for t in out)
     top = ids = None
     if top_k:
-        top = torch.empty(rows, top_k, dtype=torch.float32, device=device)
-        ids = torch.empty(rows, top_k, dtype=torch.int64, device=device)
+        top = torch.empty(*lead, top_k, dtype=torch.float32, device=device)
+        ids = torch.empty(*lead, top_k, dtype=torch.int64, device=device)
         a.top_logprobs, a.top_ids = top.data_ptr(), ids.data_ptr()
     return out[0], out[1], out[2], top, ids
 
@@ -121,11 +122,16 @@ def join_logprob_parts(stats, keys, targets, vocab_total: int, temperature: floa
                          f"{tuple(keys.shape)})")
     if t is not None and t.numel() != rows:
         raise ValueError(f"{t.numel()} targets for {rows} rows")
+    return _join(stats, keys, t, vocab_total, temperature, ignore_index, (rows,))
+
+
+def _join(stats, keys, t, vocab_total, temperature, ignore_index, lead):
+    parts, rows, top_k = keys.shape
     a = _lib.ForgeLogprobsArgs()
     a.targets = t.data_ptr() if t is not None else None
     a.rows, a.vocab_total, a.vocab, a.ld = rows, vocab_total, vocab_total, vocab_total
     a.ignore_index, a.temperature, a.top_k = ignore_index, temperature, top_k
-    res = _outputs(a, rows, top_k, stats.device)
+    res = _outputs(a, lead, top_k, stats.device)
     _call("forge_logprobs_join", stats.device, ctypes.byref(a), stats.data_ptr(), keys.data_ptr(), parts)
     return res
 
@@ -148,18 +154,15 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature, ignore_index, vocab_start, vocab_total, group):
         x, t = _rows(logits), _targets(targets)
-        a = _args(x, t, top_k, temperature, ignore_index, vocab_start, vocab_total)
+        lead = logits.shape[:-1]
         if group is None:
-            lp, ent, lse, top, ids = _outputs(a, x.shape[0], top_k, x.device)
+            a = _args(x, t, top_k, temperature, ignore_index, vocab_start, vocab_total)
+            lp, ent, lse, top, ids = _outputs(a, lead, top_k, x.device)
             _call("forge_logprobs_forward", x.device, ctypes.byref(a))
         else:
             stats, keys = logprob_parts(x, t, vocab_start, vocab_total, top_k, temperature, ignore_index)
-            lp, ent, lse, top, ids = join_logprob_parts(*_gather_parts(stats, keys, group), t, vocab_total, temperature,
-                                                        ignore_index)
-        lead = logits.shape[:-1]
-        lp, ent = lp.view(lead), ent.view(lead)
+            lp, ent, lse, top, ids = _join(*_gather_parts(stats, keys, group), t, vocab_total, temperature, ignore_index, lead)
         if top_k:
-            top, ids = top.view(*lead, top_k), ids.view(*lead, top_k)
             ctx.mark_non_differentiable(top, ids)
         ctx.set_materialize_grads(False)
         # the logits themselves where they are rows already, so that autograd notices if they are changed

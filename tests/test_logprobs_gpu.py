@@ -219,6 +219,18 @@ def test_rows_without_a_gradient_of_their_own():
             assert (dx[:5] == 0).all() and (dx[5:] != 0).any()
 
 
+def test_results_may_be_changed_in_place():
+    x, t = make(3, 50, torch.float32, seed=43)
+    x = x.requires_grad_(True)
+    for view in (x, x[:, 1:]):                         # the direct call; rows of a wider pitch
+        (want,) = torch.autograd.grad(token_logprobs(view, t.clamp(max=48)).logprobs.sum(), x)
+        out = token_logprobs(view, t.clamp(max=48), top_k=2)
+        out.logprobs.neg_()
+        out.top_logprobs.exp_()
+        (dx,) = torch.autograd.grad(out.logprobs.sum(), x)
+        assert torch.equal(dx, -want)
+
+
 def test_gradient_against_differences():
     # exact in fp32: logits of a few bits, differences of the 64-bit function
     x, t = make(2, 37, torch.float32, seed=13, spread=1.0)
