@@ -86,6 +86,8 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1, transposed: bool = False,
         rc = _lib.load().forge_fp8_quantize(ctypes.byref(a), _lib.current_stream_ptr(dev))
     if rc:
         _lib.check(rc, "forge_fp8_quantize")
+    # (for autograd: a graph that has saved these codes must not go on with other values)
+    torch.autograd.graph.increment_version([t for t in out if not t.is_inference()])
     return tuple(out)
 
 
@@ -125,8 +127,8 @@ def fp8_matmul(x_codes, x_scales, w_codes, w_scales) -> torch.Tensor:
 
 
 class Fp8Weight:
-    """Codes and scales of a weight (N, K) in 128 x 128 blocks and, for input gradients, of its transpose.  A backward pass
-    reads the transposed codes as they are then: call ``update_`` after it."""
+    """Codes and scales of a weight (N, K) in 128 x 128 blocks and, for input gradients, of its transpose, which a backward
+    pass reads: call ``update_`` after it (autograd refuses to go on with codes that have been rewritten)."""
 
     __slots__ = ("codes", "scales", "codes_t", "scales_t")
 

@@ -186,6 +186,21 @@ def test_streams_and_graph():
         assert torch.equal(p, q) and torch.equal(p, r)
 
 
+@pytest.mark.parametrize("bias", [False, True])
+def test_codes_rewritten_before_the_backward_are_noticed(bias):
+    w = torch.randn(256, 128, device=DEV)
+    fw = Fp8Weight.from_weight(w)
+    x = torch.randn(10, 128, device=DEV).bfloat16().requires_grad_(True)
+    b = torch.zeros(256, device=DEV, dtype=torch.bfloat16) if bias else None
+    y = fp8_linear(x, fw, b)
+    fw.update_(w * 2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    fp8_linear(x, fw, b).sum().backward()
+    with torch.inference_mode():
+        Fp8Weight.from_weight(w).update_(w)
+
+
 def test_refusals():
     x, w = torch.randn(8, 256, device=DEV), torch.randn(130, 256, device=DEV)
     xq, xs = quantize_fp8(x)
