@@ -166,9 +166,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     (per parameter group); ``max_grad_norm``: clip by the common norm of all gradients (``last_grad_norm`` then holds it,
     on the device).
 
-    For CUDA graphs call ``enable_device_hyper()`` and, before each captured or replayed ``step()``, ``pre_step()``: it counts
-    the step and writes the groups' hyper-parameters to device memory, where ``step()`` reads them; every parameter with
-    a gradient is then taken to be updated in every step."""
+    For CUDA graphs run one eager step, which creates the moments, call ``enable_device_hyper()`` and, before each captured
+    or replayed ``step()``, ``pre_step()``: it counts the step and writes the groups' hyper-parameters to device memory, where
+    ``step()`` reads them; every parameter with a gradient is then taken to be updated in every step."""
 
     def __init__(self, params, lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_mode: str = "f32", max_grad_norm: float | None = None):
@@ -196,6 +196,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def _state_of(self, p, mode):
         st = self.state[p]
         if not st:
+            if torch.cuda.is_current_stream_capturing():
+                del self.state[p]
+                raise RuntimeError("the moments are created (zeroed) in the first step: run one step before it is captured")
             dt, dev = _DTYPE_OF[mode], p.device
             st["step"] = 0
             st["exp_avg"] = torch.zeros(p.shape, dtype=dt, device=dev)
@@ -218,6 +221,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def _hyper_block(self, index, device):
         hd = self._device_hyper.get((index, device))
         if hd is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call pre_step() before a step and before it is captured")
             hd = self._device_hyper[(index, device)] = DeviceHyper(device)
             self._write_hyper(hd, self.param_groups[index])
         return hd

@@ -343,6 +343,23 @@ def test_replayed_steps_are_counted_in_checkpoints():
     assert opt.state_dict()["state"][0]["step"] == 4
 
 
+def test_capture_without_a_state_is_refused():
+    """A state created during a capture would be zeroed by every replay."""
+    (p, *_), opt = _params(5), None
+    opt = MultiTensorAdamW([p])
+    p.grad = torch.ones_like(p)
+    before = p.detach().clone()
+    for hyper in (False, True):
+        if hyper:
+            opt.enable_device_hyper().pre_step()
+        with pytest.raises(RuntimeError, match="before it is captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                opt.step()
+    assert not opt.state and torch.equal(p, before)
+    opt.step()
+    assert not torch.equal(p, before)
+
+
 def test_refusals():
     p, g = torch.zeros(8, 8, device=DEV), torch.zeros(8, 8, device=DEV)
     m, v = torch.zeros(8, 8, device=DEV), torch.zeros(8, 8, device=DEV)
