@@ -196,7 +196,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def _state_of(self, p, mode):
         st = self.state[p]
         if not st:
-            if torch.cuda.is_current_stream_capturing():
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
                 del self.state[p]
                 raise RuntimeError("the moments are created (zeroed) in the first step: run one step before it is captured")
             dt, dev = _DTYPE_OF[mode], p.device
