@@ -857,6 +857,8 @@ extern "C" int forge_fp8_quantize(const ForgeFp8QuantizeArgs* args, void* cuda_s
     return fail(FORGE_ERR_INVALID_ARG, "forge_fp8_quantize: transposed codes need 128 x 128 blocks, scales_t and a pitch of at least `rows`");
   if (a.ld_x < a.cols || a.ld_codes < a.cols) return fail(FORGE_ERR_SHAPE, "forge_fp8_quantize: ld_x=%lld ld_codes=%lld cols=%lld", (long long)a.ld_x, (long long)a.ld_codes, (long long)a.cols);
   if (reinterpret_cast<uintptr_t>(a.x) % (a.dtype == FORGE_DT_BF16 ? 2 : 4)) return fail(FORGE_ERR_ALIGNMENT, "forge_fp8_quantize: x is not element-aligned");
+  if (reinterpret_cast<uintptr_t>(a.scales) % 4 || (a.codes_t != nullptr && reinterpret_cast<uintptr_t>(a.scales_t) % 4))
+    return fail(FORGE_ERR_ALIGNMENT, "forge_fp8_quantize: scales are not aligned");
   fp8::QuantParams p;
   p.x = static_cast<const uint8_t*>(a.x);
   p.q = static_cast<uint8_t*>(a.codes);
@@ -890,7 +892,9 @@ static int check_product(const ForgeFp8ProductArgs& a, const char* what) {
   if (!aligned16(a.x_codes) || !aligned16(a.w_codes) || a.ld_x % 16 || a.ld_w % 16)
     return fail(FORGE_ERR_ALIGNMENT, "%s: codes must start on 16-byte boundaries and have row pitches that are multiples of 16", what);
   if (a.ld_x < a.K || a.ld_w < a.K || a.ld_y < a.N) return fail(FORGE_ERR_SHAPE, "%s: row pitch smaller than the row", what);
-  if (reinterpret_cast<uintptr_t>(a.y) % 2) return fail(FORGE_ERR_ALIGNMENT, "%s: y is not element-aligned", what);
+  if (reinterpret_cast<uintptr_t>(a.y) % 2 || reinterpret_cast<uintptr_t>(a.x_scales) % 4 || reinterpret_cast<uintptr_t>(a.w_scales) % 4 ||
+      reinterpret_cast<uintptr_t>(a.status) % 4)
+    return fail(FORGE_ERR_ALIGNMENT, "%s: y, scales or status are not element-aligned", what);
   return FORGE_OK;
 }
 

@@ -749,6 +749,10 @@ static int check(const ForgeLogprobsArgs& a, const char* what) {
   if (a.top_k > a.vocab_total) return fail(FORGE_ERR_SHAPE, "%s: top_k (%d) exceeds the vocabulary (%lld)", what, a.top_k, (long long)a.vocab_total);
   if (a.rows > 0 && (a.vocab < 1 || a.ld < a.vocab)) return fail(FORGE_ERR_SHAPE, "%s: vocab=%lld ld=%lld", what, (long long)a.vocab, (long long)a.ld);
   if (a.rows * MAX_CLUSTER > 0x7fffffffll) return fail(FORGE_ERR_SHAPE, "%s: %lld rows", what, (long long)a.rows);
+  auto off = [](const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
+  if (off(a.targets, 8) || off(a.logprobs, 4) || off(a.entropy, 4) || off(a.lse, 4) || off(a.top_logprobs, 4) || off(a.top_ids, 8) ||
+      off(a.stats, 4) || off(a.keys, 8))
+    return fail(FORGE_ERR_ALIGNMENT, "%s: targets or outputs are not element-aligned", what);
   return FORGE_OK;
 }
 
@@ -841,6 +845,8 @@ extern "C" int forge_logprobs_join(const ForgeLogprobsArgs* args, const float* s
   if (a.rows == 0) return FORGE_OK;
   if (stats == nullptr || (a.top_k > 0 && (keys == nullptr || a.top_logprobs == nullptr || a.top_ids == nullptr)))
     return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_join: null pointer");
+  if (reinterpret_cast<uintptr_t>(stats) % 4 || reinterpret_cast<uintptr_t>(keys) % 8)
+    return fail(FORGE_ERR_ALIGNMENT, "forge_logprobs_join: stats or keys are not element-aligned");
   const loss::Params p = loss::make_params(a);
   loss::logprobs_join_kernel<<<static_cast<unsigned>((a.rows + 7) / 8), 256, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
       p, stats, reinterpret_cast<const loss::u64*>(keys), parts, a.rows);
@@ -860,7 +866,8 @@ extern "C" int forge_logprobs_backward(const ForgeLogprobsArgs* args, const floa
     return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_backward: null pointer");
   if (ld_grad < a.vocab) return fail(FORGE_ERR_SHAPE, "forge_logprobs_backward: ld_grad=%lld", (long long)ld_grad);
   const int es = a.dtype == FORGE_DT_BF16 ? 2 : 4;
-  if (reinterpret_cast<uintptr_t>(a.logits) % es != 0 || reinterpret_cast<uintptr_t>(grad) % es != 0)
+  if (reinterpret_cast<uintptr_t>(a.logits) % es != 0 || reinterpret_cast<uintptr_t>(grad) % es != 0 ||
+      reinterpret_cast<uintptr_t>(g_logprob) % 4 != 0 || reinterpret_cast<uintptr_t>(g_entropy) % 4 != 0)
     return fail(FORGE_ERR_ALIGNMENT, "forge_logprobs_backward: tensors are not element-aligned");
   loss::BackParams p;
   p.logits = static_cast<const uint8_t*>(a.logits);

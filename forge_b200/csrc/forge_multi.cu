@@ -464,6 +464,8 @@ extern "C" int forge_multi_adamw(const ForgeMultiArgs* args, void* cuda_stream) 
   if (a.state_mode != FORGE_ST_F32 && a.state_mode != FORGE_ST_BF16 && a.state_mode != FORGE_ST_INT8 && a.state_mode != FORGE_ST_FP8_BLOCK)
     return fail(FORGE_ERR_UNSUPPORTED, "forge_multi_adamw: state mode %d is not built", a.state_mode);
   if (a.hyper_device == nullptr && a.hyper.step < 1) return fail(FORGE_ERR_INVALID_ARG, "step must be >= 1 (got %d)", a.hyper.step);
+  if (reinterpret_cast<uintptr_t>(a.grad_coef) % 4 || reinterpret_cast<uintptr_t>(a.hyper_device) % 8)
+    return fail(FORGE_ERR_ALIGNMENT, "forge_multi_adamw: grad_coef or hyper_device is not aligned");
   const bool quant = a.state_mode == FORGE_ST_INT8 || a.state_mode == FORGE_ST_FP8_BLOCK;
   const int ses = a.state_mode == FORGE_ST_F32 ? 4 : (a.state_mode == FORGE_ST_BF16 ? 2 : 1);
   long long total = 0;
@@ -476,7 +478,8 @@ extern "C" int forge_multi_adamw(const ForgeMultiArgs* args, void* cuda_stream) 
     if (s.param == nullptr || s.grad == nullptr || s.m == nullptr || s.v == nullptr || (quant && (s.m_scale == nullptr || s.v_scale == nullptr)))
       return fail(FORGE_ERR_INVALID_ARG, "forge_multi_adamw: tensor %d has a null pointer", i);
     if (reinterpret_cast<uintptr_t>(s.param) % (s.param_dtype == FORGE_DT_BF16 ? 2 : 4) || reinterpret_cast<uintptr_t>(s.grad) % (s.grad_dtype == FORGE_DT_BF16 ? 2 : 4) ||
-        reinterpret_cast<uintptr_t>(s.m) % ses || reinterpret_cast<uintptr_t>(s.v) % ses)
+        reinterpret_cast<uintptr_t>(s.m) % ses || reinterpret_cast<uintptr_t>(s.v) % ses ||
+        (quant && (reinterpret_cast<uintptr_t>(s.m_scale) % 4 || reinterpret_cast<uintptr_t>(s.v_scale) % 4)))
       return fail(FORGE_ERR_ALIGNMENT, "forge_multi_adamw: tensor %d is not element-aligned", i);
     total += s.numel;
   }
@@ -540,6 +543,8 @@ extern "C" int forge_multi_norm(const ForgeNormItem* items, int32_t count, doubl
   const size_t need = forge_multi_norm_scratch_bytes(items, count);
   if (need > scratch_bytes || (need > 0 && scratch == nullptr))
     return fail(FORGE_ERR_SCRATCH, "forge_multi_norm needs %zu bytes of scratch (got %zu)", need, scratch_bytes);
+  if (reinterpret_cast<uintptr_t>(norm) % 4 || reinterpret_cast<uintptr_t>(coef) % 4)
+    return fail(FORGE_ERR_ALIGNMENT, "forge_multi_norm: norm or coef is not aligned");
   if (reinterpret_cast<uintptr_t>(scratch) % sizeof(double)) return fail(FORGE_ERR_ALIGNMENT, "forge_multi_norm: scratch is not 8-byte aligned");
   if (need / sizeof(double) > static_cast<size_t>(multi::MAX_CHUNKS)) return fail(FORGE_ERR_SHAPE, "forge_multi_norm: too many elements");
   const int passes = norm_passes(norm_total(items, count));

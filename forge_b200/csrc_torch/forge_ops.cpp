@@ -232,7 +232,7 @@ py::object multi_adamw(const py::object& params, const py::object& grads, const 
     return none;
   }
   std::vector<ForgeMultiItem> items(n);
-  PointerSet seen(3 * n);
+  PointerSet seen((quant ? 5 : 3) * n);
   for (size_t i = 0; i < n; ++i) {
     const int64_t num = p[i]->numel();
     if (!plain(*p[i], dev) || !plain(*g[i], dev) || !plain(*m[i], dev) || !plain(*v[i], dev) || !float_type(*p[i]) || !float_type(*g[i]) ||
@@ -254,7 +254,9 @@ py::object multi_adamw(const py::object& params, const py::object& grads, const 
       it.m_scale = static_cast<float*>(ms[i]->mutable_data_ptr());
       it.v_scale = static_cast<float*>(vs[i]->mutable_data_ptr());
     }
-    if (num > 0 && !(seen.insert(it.param) && seen.insert(it.m) && seen.insert(it.v))) return none;
+    if (num > 0 && !(seen.insert(it.param) && seen.insert(it.m) && seen.insert(it.v) &&
+                     (!quant || (seen.insert(it.m_scale) && seen.insert(it.v_scale)))))
+      return none;
   }
   ForgeMultiArgs a = {};
   if (grad_coef.has_value() && grad_coef->defined()) {

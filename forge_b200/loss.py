@@ -54,18 +54,22 @@ def _args(x, targets, top_k, temperature, ignore_index, vocab_start, vocab_total
     return a
 
 
+def _check_targets(targets, device):
+    if targets is not None:
+        if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
+            raise ValueError(f"targets must be integers (got {targets.dtype})")
+        if targets.device != device:
+            raise ValueError("targets and logits must be on the same device")
+
+
 def _check(logits, targets, top_k, vocab_start, vocab_total):
     _require_cuda(logits, targets)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must have a last dimension of at least one column (got {tuple(logits.shape)})")
     _lib.dtype_id(logits.dtype)
-    if targets is not None:
-        if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
-            raise ValueError(f"targets must be integers (got {targets.dtype})")
-        if targets.shape != logits.shape[:-1]:
-            raise ValueError(f"targets {tuple(targets.shape)} do not match logits {tuple(logits.shape)}")
-        if targets.device != logits.device:
-            raise ValueError("targets and logits must be on the same device")
+    _check_targets(targets, logits.device)
+    if targets is not None and targets.shape != logits.shape[:-1]:
+        raise ValueError(f"targets {tuple(targets.shape)} do not match logits {tuple(logits.shape)}")
     if not 0 <= top_k <= MAX_TOP_K:
         raise ValueError(f"top_k must be 0 .. {MAX_TOP_K} (got {top_k})")
     if top_k > vocab_total:
@@ -115,6 +119,11 @@ def join_logprob_parts(stats, keys, targets, vocab_total: int, temperature: floa
     """The rows' results from the parts of all slices, ``stats`` (parts, rows, 5) and ``keys`` (parts, rows, top_k):
     ``(logprobs, entropy, lse, top_logprobs, top_ids)``, each with the rows as its first dimension."""
     _require_cuda(stats, keys, targets)
+    if keys.dim() != 3:
+        raise ValueError(f"keys must be (parts, rows, top_k) (got {tuple(keys.shape)})")
+    _check_targets(targets, stats.device)
+    if keys.device != stats.device:
+        raise ValueError("stats and keys must be on the same device")
     stats, keys, t = stats.contiguous(), keys.contiguous(), _targets(targets)
     parts, rows, top_k = keys.shape
     if stats.dtype != torch.float32 or keys.dtype != torch.int64 or tuple(stats.shape) != (parts, rows, 5):

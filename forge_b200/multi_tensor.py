@@ -86,9 +86,14 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None
 
     ``exp_avgs`` / ``exp_avg_sqs``: the moments, all of one dtype, of the parameters' sizes: fp32, bf16, int8 or
     float8_e4m3fn; the 8-bit ones with ``exp_avg_scales`` / ``exp_avg_sq_scales``, fp32, ceil(numel / 64) values each.
+    No two of the tensors that are written may overlap (one that is given twice is refused).
     ``max_norm``: multiply the gradients by ``min(1, max_norm / (norm + 1e-6))`` of their common norm, which is returned
     (an fp32 device scalar; None without ``max_norm``); ``grad_coef``: multiply them by a device scalar instead.
     ``hyper_device``: read lr, betas, eps, decay and step from a ``DeviceHyper`` block (for captured graphs)."""
+    if not isinstance(params, (list, tuple)):
+        params = list(params)
+    if hyper_device is not None and params and hyper_device.dev.device != params[0].device:
+        raise ValueError(f"hyper_device is on {hyper_device.dev.device}, the parameters are on {params[0].device}")
     nat = native.module()
     if nat is not None and (max_norm is None or max_norm > 0):
         out = nat.multi_adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, lr, beta1, beta2, eps,
@@ -139,9 +144,9 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None
                     raise ValueError(f"tensor {i}: {what} must hold {blocks} fp32 values (got {t.numel()} of {t.dtype})")
             it.m_scale, it.v_scale = ms[i].data_ptr(), vs[i].data_ptr()
         if num:
-            for q in (it.param, it.m, it.v):
+            for q in (it.param, it.m, it.v, *((it.m_scale, it.v_scale) if quant else ())):
                 if q in seen:
-                    raise ValueError(f"tensor {i}: a parameter or moment appears twice")
+                    raise ValueError(f"tensor {i}: a parameter, moment or scale tensor appears twice")
                 seen.add(q)
     norm = None
     if max_norm is not None:

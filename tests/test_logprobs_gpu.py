@@ -339,3 +339,11 @@ def test_refusals():
             token_logprobs(xx, tt, top_k=4)
     with pytest.raises(_lib.ForgeLibraryError):
         token_logprobs(x, t.cpu())
+    stats, keys = logprob_parts(x, t, 0, 100, top_k=4)
+    stats, keys = stats[None], keys[None]
+    for args in ((stats, keys, t.float(), 100), (stats, keys, t[:3], 100), (stats, keys, t.cpu(), 100), (stats.double(), keys, t, 100),
+                 (stats, keys[:, :, 0], t, 100), (stats[:, :3], keys, t, 100)):
+        with pytest.raises((ValueError, _lib.ForgeLibraryError)):
+            join_logprob_parts(*args)
+    with pytest.raises(ValueError):
+        join_logprob_parts(stats, keys, t, 3)

@@ -372,7 +372,8 @@ def test_refusals():
                      (([p], [g], [q], [q.clone()]), {}), (([p], [g], [q], [q.clone()], [s], [torch.ones(2, device=DEV)]), {}),
                      (([p], [g], [q], [q.clone()], [s], [s.double()]), {}), (([p], [g], [m], [v], [s], [s]), {}),
                      (([p, p], [g, g], [m, m.clone()], [v, v.clone()]), {}), (([p, p.clone()], [g, g], [m, m], [v, v.clone()]), {}),
-                     (([p], [g], [m], [m]), {}), (ok, dict(step=0)), (ok, dict(max_norm=0.0)), (ok, dict(max_norm=1.0, grad_coef=s)),
+                     (([p], [g], [m], [m]), {}), (([p], [g], [q], [q.clone()], [s], [s]), {}),
+                     (ok, dict(hyper_device=K.DeviceHyper(torch.device("cpu")))), (ok, dict(step=0)), (ok, dict(max_norm=0.0)), (ok, dict(max_norm=1.0, grad_coef=s)),
                      (ok, dict(grad_coef=torch.ones(2, device=DEV)))]:
         with pytest.raises(ValueError):
             multi_tensor_adamw(*args, **kw)

@@ -31,7 +31,9 @@ def logprobs(**kw):
     (dict(vocab=0), _lib.FORGE_ERR_SHAPE), (dict(ld=99), _lib.FORGE_ERR_SHAPE), (dict(vocab_start=-1), _lib.FORGE_ERR_SHAPE),
     (dict(vocab_start=1), _lib.FORGE_ERR_SHAPE), (dict(vocab_total=200), _lib.FORGE_ERR_INVALID_ARG),
     (dict(vocab_total=1 << 31, stats=P), _lib.FORGE_ERR_SHAPE), (dict(logits=None), _lib.FORGE_ERR_INVALID_ARG),
-    (dict(logits=P + 1), _lib.FORGE_ERR_ALIGNMENT), (dict(rows=1 << 31), _lib.FORGE_ERR_SHAPE),
+    (dict(logits=P + 1), _lib.FORGE_ERR_ALIGNMENT), (dict(targets=P + 4), _lib.FORGE_ERR_ALIGNMENT),
+    (dict(entropy=P + 2), _lib.FORGE_ERR_ALIGNMENT), (dict(top_k=2, top_logprobs=P, top_ids=P + 4), _lib.FORGE_ERR_ALIGNMENT),
+    (dict(top_k=2, stats=P, keys=P + 4), _lib.FORGE_ERR_ALIGNMENT), (dict(rows=1 << 31), _lib.FORGE_ERR_SHAPE),
     (dict(vocab=3, ld=3, vocab_total=3, top_k=4, top_logprobs=P, top_ids=P), _lib.FORGE_ERR_SHAPE)])
 def test_logprobs_forward_refuses(kw, code):
     assert _lib.load().forge_logprobs_forward(ctypes.byref(logprobs(**kw)), None) == code
@@ -53,10 +55,14 @@ def test_logprobs_other_entries_refuse():
     assert lib.forge_logprobs_backward(ctypes.byref(logprobs()), P, P, None, 100, None) == bad
     assert lib.forge_logprobs_backward(ctypes.byref(logprobs()), P, P, P, 99, None) == shape
     assert lib.forge_logprobs_backward(ctypes.byref(logprobs()), P, P, P + 1, 100, None) == _lib.FORGE_ERR_ALIGNMENT
+    assert lib.forge_logprobs_backward(ctypes.byref(logprobs(lse=P + 2)), P, P, P, 100, None) == _lib.FORGE_ERR_ALIGNMENT
+    assert lib.forge_logprobs_backward(ctypes.byref(logprobs()), P + 2, P, P, 100, None) == _lib.FORGE_ERR_ALIGNMENT
+    assert lib.forge_logprobs_join(ctypes.byref(logprobs()), P + 2, P, 2, None) == _lib.FORGE_ERR_ALIGNMENT
+    assert lib.forge_logprobs_join(ctypes.byref(logprobs(top_k=2, top_logprobs=P, top_ids=P)), P, P + 4, 2, None) == _lib.FORGE_ERR_ALIGNMENT
     assert lib.forge_logprobs_backward(ctypes.byref(logprobs(rows=0)), P, P, P, 100, None) == 0
 
 
-def multi(count=1, mode=_lib.ST_F32, step=1, items=True, **kw):
+def multi(count=1, mode=_lib.ST_F32, step=1, items=True, coef=None, device=None, **kw):
     arr = (_lib.ForgeMultiItem * max(count, 1))()
     for it in arr:
         for k, v in {**dict(param=P, grad=P, m=P, v=P, numel=64, param_dtype=1, grad_dtype=1), **kw}.items():
@@ -65,6 +71,7 @@ def multi(count=1, mode=_lib.ST_F32, step=1, items=True, **kw):
     a.items = arr if items else None
     a.count, a.state_mode = count, mode
     a.hyper = _lib.ForgeHyper(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, step)
+    a.grad_coef, a.hyper_device = coef, device
     a._keep = arr
     return a
 
@@ -75,6 +82,8 @@ def multi(count=1, mode=_lib.ST_F32, step=1, items=True, **kw):
     (dict(step=0), _lib.FORGE_ERR_INVALID_ARG), (dict(numel=-1), _lib.FORGE_ERR_INVALID_ARG),
     (dict(param_dtype=2), _lib.FORGE_ERR_INVALID_ARG), (dict(grad=None), _lib.FORGE_ERR_INVALID_ARG),
     (dict(mode=_lib.ST_INT8), _lib.FORGE_ERR_INVALID_ARG), (dict(param=P + 2), _lib.FORGE_ERR_ALIGNMENT),
+    (dict(mode=_lib.ST_INT8, m_scale=P, v_scale=P + 2), _lib.FORGE_ERR_ALIGNMENT),
+    (dict(coef=P + 1), _lib.FORGE_ERR_ALIGNMENT), (dict(device=P + 4), _lib.FORGE_ERR_ALIGNMENT),
     (dict(numel=1 << 50), _lib.FORGE_ERR_SHAPE)])
 def test_multi_adamw_refuses(kw, code):
     if code == _lib.FORGE_ERR_SHAPE and not torch.cuda.is_available():
@@ -98,6 +107,8 @@ def test_multi_norm_refuses():
     assert lib.forge_multi_norm(it, 1, float("nan"), P, P, P, need, None) == bad
     assert lib.forge_multi_norm(it, 1, 1.0, P, P, P, need - 1, None) == _lib.FORGE_ERR_SCRATCH
     assert lib.forge_multi_norm(it, 1, 1.0, P, P, P + 4, need, None) == _lib.FORGE_ERR_ALIGNMENT
+    assert lib.forge_multi_norm(it, 1, 1.0, P + 2, P, P, need, None) == _lib.FORGE_ERR_ALIGNMENT
+    assert lib.forge_multi_norm(it, 1, 1.0, P, P + 2, P, need, None) == _lib.FORGE_ERR_ALIGNMENT
     it[0].dtype = 9
     assert lib.forge_multi_norm(it, 1, 1.0, P, P, P, need, None) == bad
 
@@ -116,7 +127,8 @@ def fill(cls, base, kw):
     (dict(codes_t=P, block_rows=128, ld_codes_t=200), _lib.FORGE_ERR_INVALID_ARG),
     (dict(codes_t=P, scales_t=P, block_rows=128, ld_codes_t=9), _lib.FORGE_ERR_INVALID_ARG),
     (dict(ld_x=99), _lib.FORGE_ERR_SHAPE), (dict(ld_codes=99), _lib.FORGE_ERR_SHAPE), (dict(x=P + 1), _lib.FORGE_ERR_ALIGNMENT),
-    (dict(rows=0), 0), (dict(cols=0), 0)])
+    (dict(scales=P + 2), _lib.FORGE_ERR_ALIGNMENT),
+    (dict(codes_t=P, scales_t=P + 2, block_rows=128, ld_codes_t=112), _lib.FORGE_ERR_ALIGNMENT), (dict(rows=0), 0), (dict(cols=0), 0)])
 def test_quantize_refuses(kw, code):
     base = dict(x=P, rows=10, cols=100, ld_x=100, dtype=_lib.DT_BF16, block_rows=1, codes=P, ld_codes=112, scales=P)
     assert _lib.load().forge_fp8_quantize(ctypes.byref(fill(_lib.ForgeFp8QuantizeArgs, base, kw)), None) == code
@@ -126,7 +138,8 @@ def test_quantize_refuses(kw, code):
     (dict(M=-1), _lib.FORGE_ERR_INVALID_ARG), (dict(K=0), _lib.FORGE_ERR_SHAPE), (dict(K=1 << 32), _lib.FORGE_ERR_SHAPE),
     (dict(y=None), _lib.FORGE_ERR_INVALID_ARG), (dict(x_codes=P + 8), _lib.FORGE_ERR_ALIGNMENT),
     (dict(ld_w=264), _lib.FORGE_ERR_ALIGNMENT), (dict(ld_x=240), _lib.FORGE_ERR_SHAPE), (dict(ld_y=3), _lib.FORGE_ERR_SHAPE),
-    (dict(y=P + 1), _lib.FORGE_ERR_ALIGNMENT), (dict(M=0), 0), (dict(N=0), 0)])
+    (dict(y=P + 1), _lib.FORGE_ERR_ALIGNMENT), (dict(x_scales=P + 1), _lib.FORGE_ERR_ALIGNMENT), (dict(w_scales=P + 2), _lib.FORGE_ERR_ALIGNMENT),
+    (dict(status=P + 2), _lib.FORGE_ERR_ALIGNMENT), (dict(M=0), 0), (dict(N=0), 0)])
 def test_product_refuses(kw, code):
     base = dict(x_codes=P, x_scales=P, w_codes=P, w_scales=P, y=P, M=4, N=128, K=256, ld_x=256, ld_w=256, ld_y=128,
                 x_scale_row=2, x_scale_col=1, w_scale_row=2, w_scale_col=1)
