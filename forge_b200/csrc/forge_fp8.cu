@@ -593,13 +593,13 @@ static int launch_product(const CUtensorMap& tw, const CUtensorMap& tx, const Pa
 }
 
 // ---------------------------------------------------------------------------------------------
-// product, a pair of CTAs per tile of 256 tokens x 256 weight rows
+// product, a pair of CTAs per tile of 256 tokens x 256 (or 128) weight rows
 // ---------------------------------------------------------------------------------------------
 // For many tokens.  The pair's MMA (cta_group::2) reads each CTA's 128 tokens and half of the tile's weight rows from that
 // CTA's shared memory, so a CTA stages 32 KB per K block for 128 x 256 x 128 products, half of what single CTAs of
 // 128 x 128 stage per product.  Tokens are the accumulator's
 // rows: a thread's scale is then one number per K block, sx[its token, kb] sw[its 128 weight rows, kb].  Every K block
-// goes to an accumulator of its own (two of 256 columns); eight warps add it, scaled, to 128 fp32 registers each thread
+// goes to an accumulator of its own (two of 256 columns, four of 128); eight warps add it, scaled, to 128 fp32 registers each thread
 // while the tensor cores work on the next one.
 //
 // 4096 x 14336 x 4096: 228 us, 2.1 PFLOP/s.  The MMAs alone, on operands that stay in place, take 156 us; with the copies of
@@ -608,19 +608,26 @@ static int launch_product(const CUtensorMap& tw, const CUtensorMap& tx, const Pa
 // (less work per warp, but 112 registers are too few): 245 to 270 us; 32 columns per fetch instead of 16: 233 us.
 namespace pair {
 constexpr int STAGES = 5;
-constexpr int STAGE = 2 * A_BYTES;                    // 128 tokens and 128 weight rows
-constexpr int OUT_BYTES = 128 * 256 * 2;
-constexpr int SMEM = 1024 + STAGES * STAGE + OUT_BYTES;
-constexpr int GROUPS = 2;                             // epilogue warpgroups, each with 256 / GROUPS columns
-constexpr int COLS = 256 / GROUPS;
+constexpr int GROUPS = 2;                             // epilogue warpgroups, each with half of the columns
 constexpr int THREADS = 128 + GROUPS * 128;           // producer, MMA, two idle warps; the epilogue
 constexpr int TMEM_COLS = 512;
+
+// W: weight rows of a tile
+template <int W>
+struct Cfg {
+  static constexpr int B_BYTES = W / 2 * BK;          // each CTA's half of them
+  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int COLS = W / GROUPS;
+  static constexpr int ACCS = TMEM_COLS / W;          // accumulators
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 128 * W * 2;
+};
+constexpr int MAX_ACCS = 4;
 
 struct Ctrl {
   uint64_t full[STAGES];
   uint64_t empty[STAGES];
-  uint64_t acc_full[2];
-  uint64_t acc_empty[2];
+  uint64_t acc_full[MAX_ACCS];
+  uint64_t acc_empty[MAX_ACCS];
   uint32_t tmem_base;
   int abort_word;
 };
@@ -639,16 +646,20 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, u
 
 constexpr int STEP = 16;                              // columns fetched from tensor memory at a time
 // acc += s * STEP columns of the accumulator
-__device__ __forceinline__ void add_scaled(float2 (&acc)[COLS / 2], int at, const uint32_t (&r)[STEP], float s) {
+template <int N>
+__device__ __forceinline__ void add_scaled(float2 (&acc)[N], int at, const uint32_t (&r)[STEP], float s) {
   const float2 s2 = make_float2(s, s);
 #pragma unroll
   for (int j = 0; j < STEP / 2; ++j)
     acc[at + j] = ffma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[at + j]);
 }
 
+template <int W>
 __global__ void __launch_bounds__(THREADS, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                 const __grid_constant__ CUtensorMap tm_out, const Params p) {
+  constexpr int STAGE = Cfg<W>::STAGE, COLS = Cfg<W>::COLS, ACCS = Cfg<W>::ACCS;
+  static_assert(ACCS <= MAX_ACCS, "one barrier pair per accumulator");
   __shared__ Ctrl ctrl;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* data = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -657,11 +668,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   volatile int* abort_word = &ctrl.abort_word;
   const uint32_t cta_rank = cluster_ctarank();
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(gridDim.x) / 2;
-  const int num_tiles = p.tiles_m * ((p.N + 255) / 256);
+  const int num_tiles = p.tiles_m * ((p.N + W - 1) / W);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) { mbar_init(&ctrl.full[i], 1); mbar_init(&ctrl.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&ctrl.acc_full[i], 1); mbar_init(&ctrl.acc_empty[i], 8 * GROUPS); }
+    for (int i = 0; i < ACCS; ++i) { mbar_init(&ctrl.acc_full[i], 1); mbar_init(&ctrl.acc_empty[i], 8 * GROUPS); }
     ctrl.abort_word = 0;
     mbar_fence_init();
   }
@@ -688,7 +699,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       int it = 0;
       for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
         const int m0 = (tile % p.tiles_m) * 256 + static_cast<int>(cta_rank) * 128;
-        const int n0 = (tile / p.tiles_m) * 256 + static_cast<int>(cta_rank) * 128;
+        const int n0 = (tile / p.tiles_m) * W + static_cast<int>(cta_rank) * (W / 2);
         for (int kb = 0; kb < p.KB; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&ctrl.empty[s], ((it / STAGES) & 1) ^ 1, abort_word, ERR_OP_EMPTY)) goto done;
@@ -701,18 +712,18 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         }
       }
     } else if (warp == 1 && lane == 0 && cta_rank == 0) {
-      constexpr uint32_t idesc = make_idesc_e4m3(256, 256);
+      constexpr uint32_t idesc = make_idesc_e4m3(256, W);
       int it = 0;
       for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
         for (int kb = 0; kb < p.KB; ++kb, ++it) {
-          const int s = it % STAGES, b = it & 1;
-          if (!mbar_wait(&ctrl.acc_empty[b], ((it >> 1) & 1) ^ 1, abort_word, ERR_ACC_EMPTY)) goto done;
+          const int s = it % STAGES, b = it % ACCS;
+          if (!mbar_wait(&ctrl.acc_empty[b], ((it / ACCS) & 1) ^ 1, abort_word, ERR_ACC_EMPTY)) goto done;
           if (!mbar_wait(&ctrl.full[s], (it / STAGES) & 1, abort_word, ERR_OP_FULL)) goto done;
           tc_fence_after();
           const uint32_t a_addr = smem_u32(data + s * STAGE), b_addr = a_addr + A_BYTES;
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
-            umma_f8_pair(tmem_base + b * 256, make_smem_desc_sw128(a_addr + k * 32, 16, 1024),
+            umma_f8_pair(tmem_base + b * W, make_smem_desc_sw128(a_addr + k * 32, 16, 1024),
                          make_smem_desc_sw128(b_addr + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
           umma_commit_pair(&ctrl.empty[s], 3);
           umma_commit_pair(&ctrl.acc_full[b], 3);
@@ -724,13 +735,13 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     const int quarter = warp & 3, group = (warp - 4) >> 2;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + group * COLS;
     uint8_t* stage = out_buf + (group * 4 + quarter) * (32 * COLS * 2);          // boxes of 32 rows x 64 columns
-    const uint32_t empty_leader0 = map_to_cta(smem_u32(&ctrl.acc_empty[0]), 0), empty_leader1 = map_to_cta(smem_u32(&ctrl.acc_empty[1]), 0);
+    const uint32_t empty_leader = map_to_cta(smem_u32(&ctrl.acc_empty[0]), 0);
     const uint64_t pol = policy_evict_normal();
     if (p.early) wait_for_previous();
     int it = 0;
     for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
       const int row = (tile % p.tiles_m) * 256 + static_cast<int>(cta_rank) * 128 + quarter * 32 + lane;
-      const int col = (tile / p.tiles_m) * 256 + group * COLS;
+      const int col = (tile / p.tiles_m) * W + group * COLS;
       const bool live = row < p.M && col < p.N;
       const float* sx = p.sx + static_cast<long long>(live ? row : 0) * p.sx_row;
       const float* sw = p.sw + static_cast<long long>(live ? col / 128 : 0) * p.sw_row;
@@ -748,7 +759,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       for (int j = 0; j < COLS / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
       for (int kb = 0; kb < p.KB; ++kb, ++it) {
-        const int b = it & 1;
+        const int b = it % ACCS;
         const float s = s0.x * s0.y;
         s0 = s1;
         if (live && kb + 2 < p.KB) {
@@ -756,11 +767,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           sx += p.sx_col;
           sw += p.sw_col;
         }
-        bool ok = mbar_wait(&ctrl.acc_full[b], (it >> 1) & 1, abort_word, ERR_ACC_FULL);
+        bool ok = mbar_wait(&ctrl.acc_full[b], (it / ACCS) & 1, abort_word, ERR_ACC_FULL);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) goto done;
         tc_fence_after();
-        const uint32_t ta = lane_addr + b * 256;
+        const uint32_t ta = lane_addr + b * W;
         // two fetches in flight: each is asked for again as soon as its columns have been added
         uint32_t r0[STEP], r1[STEP];
         tmem_ld_32x16(ta, r0);
@@ -771,7 +782,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           if (c + 2 * STEP >= COLS) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(b ? empty_leader1 : empty_leader0);
+            if (lane == 0) mbar_arrive_cluster(empty_leader + b * 8);
           }
           add_scaled(acc, c / 2, r0, s);
           if (c + 2 * STEP < COLS) tmem_ld_32x16(ta + c + 2 * STEP, r0);
@@ -828,13 +839,14 @@ done:
   }
 }
 
+template <int W>
 static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& ty, const Params& p, int pairs, int device,
                   cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  const int rc = allow_smem(fp8_pair_kernel, SMEM, done, device);
+  const int rc = allow_smem(fp8_pair_kernel<W>, Cfg<W>::SMEM, done, device);
   if (rc != FORGE_OK) return rc;
-  Launch l(2 * pairs, THREADS, SMEM, 2, p.early, stream);
-  cudaError_t e = cudaLaunchKernelEx(&l.cfg, fp8_pair_kernel, tx, tw, ty, p);
+  Launch l(2 * pairs, THREADS, Cfg<W>::SMEM, 2, p.early, stream);
+  cudaError_t e = cudaLaunchKernelEx(&l.cfg, fp8_pair_kernel<W>, tx, tw, ty, p);
   if (e != cudaSuccess) return fail(FORGE_ERR_CUDA, "fp8 product launch: %s", cudaGetErrorString(e));
   return FORGE_OK;
 }
@@ -925,13 +937,17 @@ static int run_product(const ForgeFp8ProductArgs& a, bool early, cudaStream_t st
 
   // Pairs of CTAs where they need fewer rounds of K blocks over the GPU than the tiles of 128 x 128, a round taking about
   // as long in both (0.55 us).  With K = 4096, pairs / tiles: 256 x 14336 23.5 / 42 us, 512 x 14336 39 / 78,
-  // 4096 x 14336 228 / 478, 512 x 4096 22 / 23, 512 x 1024 20 / 13.5 (K cut in four), 128 x 4096 21 / 14.
-  const int64_t pair_tiles = ((a.M + 255) / 256) * ((a.N + 255) / 256), pair_slots = di->sm_count / 2;
-  const int64_t pair_time = (pair_tiles + pair_slots - 1) / pair_slots * p.KB;
+  // 4096 x 14336 228 / 478, 512 x 1024 20 / 13.5 (K cut in four), 128 x 4096 21 / 14.  Tiles of half the weight rows where
+  // one round holds them, a round taking three quarters as long: 512 x 4096 19.5 us, 22.7 without, with K = 14336 53 and 61.
+  // (As the last, partial round of many tiles they are not worth it: a kernel that does both is 2 % slower per whole tile.)
+  const int64_t tiles_m = (a.M + 255) / 256, pair_slots = di->sm_count / 2;
+  const int64_t pair_tiles = tiles_m * ((a.N + 255) / 256), half_tiles = tiles_m * ((a.N + 127) / 128);
+  const bool halves = half_tiles <= pair_slots;
+  const int64_t pair_time = halves ? p.KB * 3 / 4 : (pair_tiles + pair_slots - 1) / pair_slots * p.KB;
   const int64_t tile_time = (tiles * p.split + slots - 1) / slots * ((p.KB + p.split - 1) / p.split);
   const bool pairs = nt == 128 && pair_time < tile_time;
   CUtensorMap tw, tx, ty;
-  int rc = encode_tmap_2d(&tw, a.w_codes, 1, false, a.N, a.K, a.ld_w, fp8::BK, 128, 128);
+  int rc = encode_tmap_2d(&tw, a.w_codes, 1, false, a.N, a.K, a.ld_w, fp8::BK, pairs && halves ? 64 : 128, 128);
   if (rc != FORGE_OK) return rc;
   rc = encode_tmap_2d(&tx, a.x_codes, 1, false, a.M, a.K, a.ld_x, fp8::BK, nt, 128);
   if (rc != FORGE_OK) return rc;
@@ -941,9 +957,10 @@ static int run_product(const ForgeFp8ProductArgs& a, bool early, cudaStream_t st
       rc = encode_tmap_2d(&ty, a.y, 2, true, a.M, a.N, a.ld_y, 64, 32, 128);
       if (rc != FORGE_OK) return rc;
     }
-    p.tiles_m = static_cast<int>((a.M + 255) / 256);
+    p.tiles_m = static_cast<int>(tiles_m);
     p.split = 1;
-    return fp8::pair::launch(tx, tw, ty, p, static_cast<int>(std::min<int64_t>(pair_tiles, pair_slots)), di->device, stream);
+    if (halves) return fp8::pair::launch<128>(tx, tw, ty, p, static_cast<int>(half_tiles), di->device, stream);
+    return fp8::pair::launch<256>(tx, tw, ty, p, static_cast<int>(std::min<int64_t>(pair_tiles, pair_slots)), di->device, stream);
   }
   const int ctas = static_cast<int>(tiles * p.split);
   switch (nt) {

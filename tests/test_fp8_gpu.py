@@ -91,7 +91,8 @@ def check_product(xq, xs, wq, ws, y):
 
 @pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 1, 1), (1, 1030, 4096), (1, 20000, 700), (2, 5000, 1040), (2, 130, 300), (3, 777, 5000), (4, 6000, 514), (4, 129, 16), (5, 20001, 1168), (8, 4100, 2064), (7, 33, 130), (16, 256, 512), (17, 129, 1000), (33, 640, 144),
                                    (64, 1024, 2048), (65, 257, 384), (128, 128, 128), (129, 300, 520), (200, 1024, 7168), (500, 2000, 640),
-                                   (512, 4096, 1024), (700, 515, 260), (1100, 3000, 900), (5, 14336, 4096), (2048, 1024, 256)])
+                                   (512, 4096, 1024), (700, 515, 260), (1100, 3000, 900), (5, 14336, 4096), (2048, 1024, 256),
+                                   (300, 4090, 1000), (390, 4072, 640), (1500, 1000, 300)])
 def test_product_against_64_bits(m, n, k):
     g = torch.Generator(device=DEV).manual_seed(m + n + k)
     x = torch.randn(m, k, device=DEV, generator=g)
