@@ -208,6 +208,33 @@ bool plain(const at::Tensor& t, int dev) {
   return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous();
 }
 
+// norm and (max_norm > 0) the factor that clips to it, as two elements of one tensor
+at::Tensor norm_of(const std::vector<ForgeNormItem>& items, double max_norm, const at::Tensor& like, void* stream) {
+  const int32_t n = static_cast<int32_t>(items.size());
+  const size_t bytes = forge_multi_norm_scratch_bytes(items.data(), n);
+  at::Tensor out = empty({2}, at::kFloat, like), scratch = empty({static_cast<int64_t>(bytes + 8)}, at::kByte, like);
+  float* o = static_cast<float*>(out.data_ptr());
+  check(forge_multi_norm(items.data(), n, max_norm, o, max_norm > 0 ? o + 1 : nullptr, scratch.data_ptr(), bytes, stream), "forge_multi_norm");
+  return out;
+}
+
+// None: not of the plain form.  Otherwise (norm, factor or None).
+py::object multi_norm(const py::object& grads, double max_norm) {
+  const py::object none = py::none();
+  std::vector<const at::Tensor*> g;
+  if (!unpack(grads, g) || g.empty() || !g[0]->is_cuda()) return none;
+  const int dev = g[0]->get_device();
+  std::vector<ForgeNormItem> items(g.size());
+  for (size_t i = 0; i < g.size(); ++i) {
+    if (!plain(*g[i], dev) || !float_type(*g[i])) return none;
+    items[i] = ForgeNormItem{g[i]->const_data_ptr(), g[i]->numel(), dtype_id(*g[i]), 0};
+  }
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+  const at::Tensor out = norm_of(items, max_norm, *g[0], stream_of(dev));
+  auto wrap = [](const at::Tensor& v) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(v)); };
+  return py::make_tuple(wrap(out.select(0, 0)), max_norm > 0 ? wrap(out.select(0, 1)) : none);
+}
+
 // None: not of the plain form.  Otherwise (done, norm or None).
 py::object multi_adamw(const py::object& params, const py::object& grads, const py::object& exp_avgs, const py::object& exp_avg_sqs,
                        const py::object& m_scales, const py::object& v_scales, double lr, double beta1, double beta2, double eps,
@@ -265,16 +292,12 @@ py::object multi_adamw(const py::object& params, const py::object& grads, const 
   }
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
   void* stream = stream_of(dev);
-  at::Tensor out, scratch;
+  at::Tensor out;
   if (max_norm > 0) {
     std::vector<ForgeNormItem> gi(n);
     for (size_t i = 0; i < n; ++i) gi[i] = ForgeNormItem{items[i].grad, items[i].numel, items[i].grad_dtype, 0};
-    const size_t bytes = forge_multi_norm_scratch_bytes(gi.data(), static_cast<int32_t>(n));
-    out = empty({2}, at::kFloat, *p[0]);
-    scratch = empty({static_cast<int64_t>(bytes + 8)}, at::kByte, *p[0]);
-    float* o = static_cast<float*>(out.data_ptr());
-    check(forge_multi_norm(gi.data(), static_cast<int32_t>(n), max_norm, o, o + 1, scratch.data_ptr(), bytes, stream), "forge_multi_norm");
-    a.grad_coef = o + 1;
+    out = norm_of(gi, max_norm, *p[0], stream);
+    a.grad_coef = static_cast<float*>(out.data_ptr()) + 1;
   }
   a.items = items.data();
   a.count = static_cast<int32_t>(n);
@@ -417,6 +440,7 @@ py::object quantize(const at::Tensor& x, int64_t block_rows, bool transposed) {
 void bind_operators(pybind11::module_& m) {
   m.def("token_logprobs", &token_logprobs);
   m.def("multi_adamw", &multi_adamw);
+  m.def("multi_norm", &multi_norm);
   m.def("fp8_linear", &fp8_linear);
   m.def("fp8_quantize", &quantize);
   m.def("set_status_word", [](int64_t device, int64_t ptr) {

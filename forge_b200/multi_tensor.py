@@ -57,6 +57,11 @@ def _one_device(tensors):
 def multi_tensor_grad_norm(grads, max_norm: float | None = None):
     """``(norm, coef)`` of a list of CUDA gradients, fp32 scalars on their device: the 2-norm of all elements and, with
     ``max_norm``, ``min(1, max_norm / (norm + 1e-6))`` (None without).  Bit-reproducible; no host synchronisation."""
+    nat = native.module()
+    if nat is not None and (max_norm is None or max_norm > 0):
+        out = nat.multi_norm(grads, max_norm or 0.0)
+        if out is not None:
+            return out
     grads = _grads(grads)
     if max_norm is not None and not max_norm > 0:
         raise ValueError(f"max_norm must be positive (got {max_norm})")
@@ -270,25 +275,32 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         for index, group in enumerate(self.param_groups):
             self._check_group(group)
             # one call per device and step count (a parameter without a gradient in some step counts its own steps)
-            calls: dict[tuple, list] = {}
+            calls: dict[tuple, tuple] = {}
+            mode = group["state_mode"]
             for p in group["params"]:
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                st = self._state_of(p, group["state_mode"])
-                if self._device_hyper is not None:
-                    st["step"] = self._device_step
-                else:
-                    st["step"] += 1
-                calls.setdefault((p.device, st["step"], st["exp_avg"].dtype), []).append((p, st))
+                st = self.state[p] or self._state_of(p, mode)
+                count = st["step"] = st["step"] + 1 if self._device_hyper is None else self._device_step
+                m = st["exp_avg"]
+                key = p.device, count, m.dtype
+                lists = calls.get(key)
+                if lists is None:
+                    lists = calls[key] = [], [], [], [], [], []
+                lists[0].append(p)
+                lists[1].append(grad)
+                lists[2].append(m)
+                lists[3].append(st["exp_avg_sq"])
+                if m.dtype in _QUANTIZED:
+                    lists[4].append(st["exp_avg_scale"])
+                    lists[5].append(st["exp_avg_sq_scale"])
             b1, b2 = group["betas"]
-            for (dev, count, sdt), members in calls.items():
-                quant = sdt in _QUANTIZED
-                multi_tensor_adamw(
-                    [p.detach() for p, _ in members], [p.grad for p, _ in members], [s["exp_avg"] for _, s in members],
-                    [s["exp_avg_sq"] for _, s in members], [s["exp_avg_scale"] for _, s in members] if quant else None,
-                    [s["exp_avg_sq_scale"] for _, s in members] if quant else None, lr=group["lr"], beta1=b1, beta2=b2,
-                    eps=group["eps"], weight_decay=group["weight_decay"], step=max(count, 1), grad_coef=coefs.get(dev),
-                    hyper_device=self._hyper_block(index, dev) if self._device_hyper is not None else None)
+            for (dev, count, sdt), lists in calls.items():
+                multi_tensor_adamw(*lists[:4 if sdt not in _QUANTIZED else 6], lr=group["lr"], beta1=b1, beta2=b2,
+                                   eps=group["eps"], weight_decay=group["weight_decay"], step=max(count, 1),
+                                   grad_coef=coefs.get(dev),
+                                   hyper_device=self._hyper_block(index, dev) if self._device_hyper is not None else None)
         return loss
 
     def load_state_dict(self, state_dict):
