@@ -220,7 +220,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         return st
 
     def enable_device_hyper(self):
-        self._device_hyper = {}
+        if self._device_hyper is None:             # (captured steps read the blocks that are there)
+            self._device_hyper = {}
         self._device_step = max((st["step"] for st in self.state.values() if st), default=0)
         return self
 
@@ -303,14 +304,25 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                                    hyper_device=self._hyper_block(index, dev) if self._device_hyper is not None else None)
         return loss
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """As in ``torch.optim``, but the moments keep the types they were saved in (the base class would cast them to the
-        parameters' type)."""
+        parameters' type), and are loaded into the tensors that are there where those fit: a captured ``step()`` goes on
+        with them."""
+        there = dict(self.state)
         super().load_state_dict(state_dict)
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, index in zip(group["params"], saved["params"]):
                 st = state_dict["state"].get(index)
                 if st:
-                    self.state[p] = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else copy.deepcopy(v)
-                                     for k, v in st.items()}
+                    old = there.get(p, {})
+                    self.state[p] = {k: self._load(old.get(k), v, p.device) for k, v in st.items()}
         self._device_step = max((st["step"] for st in self.state.values() if st), default=0)
+
+    @staticmethod
+    def _load(old, new, device):
+        if not isinstance(new, torch.Tensor):
+            return copy.deepcopy(new)
+        if isinstance(old, torch.Tensor) and old.shape == new.shape and old.dtype == new.dtype and old.device == device:
+            return old.copy_(new)
+        return new.to(device, copy=True)

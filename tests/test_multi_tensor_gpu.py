@@ -343,6 +343,38 @@ def test_replayed_steps_are_counted_in_checkpoints():
     assert opt.state_dict()["state"][0]["step"] == 4
 
 
+def test_a_captured_step_goes_on_with_a_loaded_checkpoint():
+    a, b = _params(6, torch.bfloat16), _params(6, torch.bfloat16)
+    opt, ref = MultiTensorAdamW(a, lr=1e-2, state_mode="int8"), MultiTensorAdamW(b, lr=1e-2, state_mode="int8")
+    for ps in (a, b):
+        _give_grads(ps, 0)
+    opt.step()
+    ref.step()
+    saved = copy.deepcopy(opt.state_dict()), [p.detach().clone() for p in a]
+    opt.enable_device_hyper()
+    graph = torch.cuda.CUDAGraph()
+    opt.pre_step()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+        opt.pre_step()
+    opt.load_state_dict(saved[0])
+    opt.enable_device_hyper()                         # (again: what the graph reads stays where it is)
+    with torch.no_grad():
+        for p, q in zip(a, saved[1]):
+            p.copy_(q)
+    for _ in range(2):
+        opt.pre_step()
+        graph.replay()
+        ref.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+        for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"):
+            u, v = opt.state[p][k], ref.state[q][k]
+            assert torch.equal(u, v) if isinstance(u, torch.Tensor) else u == v
+
+
 def test_capture_without_a_state_is_refused():
     """A state created during a capture would be zeroed by every replay."""
     (p, *_), opt = _params(5), None
