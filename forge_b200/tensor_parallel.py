@@ -231,7 +231,7 @@ class RowShardedLinearSet(nn.Module):
         for m in self.members:
             loc = m.local
             if not (m.world > 1 and loc.training and loc._config is not None and not loc._is_accumulating
-                    and loc.use_fused_backward and loc.bias is None and loc.weight.dtype == torch.bfloat16):
+                    and loc.use_fused_backward and not loc.fp8_products and loc.bias is None and loc.weight.dtype == torch.bfloat16):
                 return False
             loc._ensure_state()
             if loc._state._pending_grad is not None:
@@ -311,7 +311,7 @@ class RowShardedFusedLinear(nn.Module):
     def _fused_conditions(self, x) -> bool:
         loc = self.local
         if not (self.gather_input and self.world > 1 and loc.training and loc._config is not None
-                and not loc._is_accumulating and loc.use_fused_backward and loc.bias is None and x.is_cuda
+                and not loc._is_accumulating and loc.use_fused_backward and not loc.fp8_products and loc.bias is None and x.is_cuda
                 and x.dtype == torch.bfloat16 and loc.weight.dtype == torch.bfloat16):
             return False
         loc._ensure_state()

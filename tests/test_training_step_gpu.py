@@ -200,6 +200,23 @@ def test_fp8_products_of_a_fused_linear(bias):
         FusedLinear(64, 64).half().use_fp8_products()
 
 
+def test_fp8_products_of_a_row_sharded_linear_take_the_plain_path():
+    """The forms that fuse a collective into the GEMM multiply the weight as it is: a linear with 8-bit products has none."""
+    from forge_b200.tensor_parallel import RowShardedFusedLinear, RowShardedLinearSet
+    x = torch.zeros(2, 32, device=DEV, dtype=torch.bfloat16)
+    lin = RowShardedFusedLinear(64, 64, rank=0, world=2, dtype=torch.bfloat16, device=DEV, bias=False).train()
+    part = RowShardedFusedLinear(64, 64, rank=0, world=2, gather_input=False, dtype=torch.bfloat16, device=DEV, bias=False).train()
+    both = RowShardedLinearSet([part])
+    both.attach_fused_scatter(object(), 0)            # only asked for by what runs fused
+    lin.attach_fused_gather(object(), 0)
+    for m in (lin, part):
+        m.local.update_optimizer_config(OptimizerConfig(lr=1e-3))
+    assert lin.returns_full_output(x) and both.fused(x)
+    for m in (lin, part):
+        m.local.use_fp8_products()
+    assert not lin.returns_full_output(x) and not both.fused(x)
+
+
 def test_sharded_loss_of_one_rank_equals_the_torch_ops():
     from examples.tp_model import _VocabParallelCrossEntropy, library_cross_entropy
     dist.init_process_group("nccl", rank=0, world_size=1, store=dist.HashStore(), device_id=torch.device(DEV, 0))
