@@ -12,7 +12,7 @@ from forge_b200 import FusedLinear, FusedOptimizerManager, OptimizerConfig
 from forge_b200 import kernel as K
 from forge_b200.fp8 import Fp8Weight, fp8_linear
 from forge_b200.loss import token_logprobs
-from forge_b200.multi_tensor import MultiTensorAdamW
+from forge_b200.multi_tensor import MultiTensorAdamW, multi_tensor_adamw
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -215,6 +215,48 @@ def test_fp8_products_of_a_row_sharded_linear_take_the_plain_path():
     for m in (lin, part):
         m.local.use_fp8_products()
     assert not lin.returns_full_output(x) and not both.fused(x)
+
+
+def test_calls_from_several_threads_and_streams():
+    import threading
+    torch.manual_seed(9)
+    x = torch.randn(70, 33000, device=DEV).bfloat16()
+    t = torch.randint(0, 33000, (70,), device=DEV)
+    w = torch.randn(1000, 512, device=DEV).bfloat16()
+    a = [torch.randn(n, 512, device=DEV).bfloat16() for n in (1, 40, 700)]
+    g = [torch.randn(n, device=DEV) for n in (5, 4096, 100000)]
+
+    def work():
+        out = []
+        for _ in range(6):
+            xr = x.detach().requires_grad_(True)
+            o = token_logprobs(xr, t, top_k=5)
+            out += [*o, torch.autograd.grad(o.logprobs.sum() + o.entropy.sum(), xr)[0]]
+            w8 = Fp8Weight.from_weight(w)
+            out += [fp8_linear(v, w8) for v in a]
+            p, m, v = ([torch.zeros_like(u) for u in g] for _ in range(3))
+            out.append(multi_tensor_adamw(p, g, m, v, max_norm=1.0))
+            out += p
+        return [o.detach() for o in out]
+
+    want = work()
+    torch.cuda.synchronize()
+    results = {}
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            results[i] = work()
+        s.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert len(results) == 4
+    for got in results.values():
+        assert len(got) == len(want) and all(torch.equal(p, q) for p, q in zip(got, want))
 
 
 def test_sharded_loss_of_one_rank_equals_the_torch_ops():
