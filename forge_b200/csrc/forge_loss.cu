@@ -1,8 +1,10 @@
 // Log probability of one given token per row of logits, the row's entropy and its most likely
 // alternatives, and the gradient of the first two with respect to the logits.  With z = x / temperature
-// and m any number near the row's maximum:
-//   S = sum e^(z - m)      T = sum (z - m) e^(z - m)      lse = m + log S
-//   logprob = z_t - lse    entropy = log S - T / S        p_j = e^(z_j - lse)
+// and m any number near the row's maximum, of the logits as they are:
+//   e_j = e^((x_j - m) / temperature)      S = sum e_j      T = sum (x_j - m) e_j      lse = m / temperature + log S
+//   logprob = (x_t - m) / temperature - log S      entropy = log S - T / (S temperature)      p_j = e^(z_j - lse)
+// Everything but lse is formed from differences of logits: m / temperature need not even be finite (logits of the
+// type's lowest value at a temperature below 1).
 //   dx_j = ( g_l (1[j = t] - p_j) - g_h p_j (log p_j + entropy) ) / temperature
 //
 // Forward: ONE pass over the logits.  Every thread keeps a running (m, S, T) of its own; m moves only
@@ -53,7 +55,7 @@ struct Params {
   float* lse;
   float* top_logprobs;
   long long* top_ids;
-  float* stats;                          // partial mode: (rows, 5) = m, S, T, target's z, target found
+  float* stats;                          // partial mode: (rows, 5) = m, S, T, target's logit, target found
   unsigned long long* keys;              // partial mode: (rows, top_k)
   long long vocab, ld, ignore_index, vocab_start, vocab_total;
   int top_k;
@@ -61,7 +63,7 @@ struct Params {
 };
 
 struct Acc {
-  float m, s, t;                         // m in units of z
+  float m, s, t;                         // m and t in units of the logits
 };
 
 // a NaN stays a NaN (fmaxf would drop it)
@@ -77,13 +79,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 // (m, S, T) of two disjoint sets of columns -> of their union.  A set without a finite logit has m = -inf
-// and S = T = 0 (or NaN, if it holds a NaN): it must not enter the differences below.
-__device__ __forceinline__ Acc join(const Acc& a, const Acc& b) {
+// and S = T = 0 (or NaN, if it holds a NaN): it must not enter the differences below.  c: log2 e / temperature.
+__device__ __forceinline__ Acc join(const Acc& a, const Acc& b, float c) {
   if (a.m == -INFINITY) return Acc{b.m, a.s + b.s, a.t + b.t};
   if (b.m == -INFINITY) return Acc{a.m, a.s + b.s, a.t + b.t};
   const float m = fmaxf(a.m, b.m);
   const float da = a.m - m, db = b.m - m;
-  const float fa = exp2_approx(da * LOG2E), fb = exp2_approx(db * LOG2E);
+  const float fa = exp2_approx(da * c), fb = exp2_approx(db * c);
   // one of da, db is zero; the other may be so low that its factor is 0, and 0 * -inf would be NaN
   const float ta = fa > 0.0f ? fa * (a.t + da * a.s) : 0.0f * a.s;
   const float tb = fb > 0.0f ? fb * (b.t + db * b.s) : 0.0f * b.s;
@@ -91,12 +93,12 @@ __device__ __forceinline__ Acc join(const Acc& a, const Acc& b) {
 }
 
 // over the lanes of a warp: the maximum first, then plain sums
-__device__ __forceinline__ Acc warp_join(const Acc& a) {
+__device__ __forceinline__ Acc warp_join(const Acc& a, float c) {
   float m = a.m, s = a.s, t = a.t;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (a.m != -INFINITY) {
-    const float d = a.m - m, f = exp2_approx(d * LOG2E);
+    const float d = a.m - m, f = exp2_approx(d * c);
     t = f > 0.0f ? f * (t + d * s) : 0.0f * s;
     s *= f;
   }
@@ -173,9 +175,9 @@ __device__ __forceinline__ u64 warp_merge(u64 a, u64 b, int lane) {
 
 // ----- one thread's running sums ------------------------------------------------------------------
 struct Run {
-  float m, thr;                          // m in raw logit units; rescale when a value exceeds thr
+  float m, thr;                          // rescale when a value exceeds thr
   float nm;                              // -m, or 0 while there is no finite logit
-  float2 s, t;                           // two interleaved partial sums; t in raw logit units
+  float2 s, t;                           // two interleaved partial sums
 };
 
 __device__ __forceinline__ void rebase(Run& r, float vmax, float lazy, float c) {
@@ -326,21 +328,21 @@ __device__ __forceinline__ void rank_keys(const u64* cand, int n, u64* best) {
   __syncthreads();
 }
 
-// what the joined row comes to; `keys` of warp 0's lanes
-__device__ __forceinline__ void write_row(const Params& p, long long row, const Acc& a, float zt, bool found, bool top,
+// what the joined row comes to; xt: the target's logit, `list`: the keys, over the lanes
+__device__ __forceinline__ void write_row(const Params& p, long long row, const Acc& a, float xt, bool found, bool top,
                                           u64 list, int lane) {
   const float log_s = logf(a.s);
   if (lane == 0) {
     const long long t = p.targets ? p.targets[row] : p.ignore_index;
     const bool ignored = p.targets == nullptr || t == p.ignore_index;
-    if (p.logprobs) p.logprobs[row] = ignored ? 0.0f : (found ? (zt - a.m) - log_s : NAN);
-    if (p.entropy) p.entropy[row] = log_s - a.t / a.s;
-    if (p.lse) p.lse[row] = a.m + log_s;
+    if (p.logprobs) p.logprobs[row] = ignored ? 0.0f : (found ? (xt - a.m) * p.inv_t - log_s : NAN);
+    if (p.entropy) p.entropy[row] = log_s - a.t / a.s * p.inv_t;
+    if (p.lse) p.lse[row] = a.m * p.inv_t + log_s;
   }
   if (top && lane < p.top_k) {
     // fewer than k comparable logits (NaN): any valid column
     p.top_ids[row * p.top_k + lane] = list != 0 ? static_cast<long long>(key_index(list)) : lane;
-    p.top_logprobs[row * p.top_k + lane] = ((list != 0 ? key_value(list) : NAN) * p.inv_t - a.m) - log_s;
+    p.top_logprobs[row * p.top_k + lane] = ((list != 0 ? key_value(list) : NAN) - a.m) * p.inv_t - log_s;
   }
 }
 
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Pa
   const long long t = p.targets ? p.targets[row] : p.ignore_index;
   const long long tl = t - p.vocab_start;
   const bool found = rank == 0 && t != p.ignore_index && t >= 0 && t < p.vocab_total && tl >= 0 && tl < p.vocab;
-  const float zt = found ? V::one(base + tl * ES) * p.inv_t : 0.0f;
+  const float xt = found ? V::one(base + tl * ES) : 0.0f;
 
   constexpr int U = 4;
   float bound = -INFINITY;               // nothing below it can be among the best k
@@ -550,12 +552,11 @@ __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Pa
     }
   }
 
-  // raw units -> units of z
-  Acc a{r.m == -INFINITY ? r.m : r.m * p.inv_t, r.s.x + r.s.y, (r.t.x + r.t.y) * p.inv_t};
-  a = warp_join(a);
+  Acc a{r.m, r.s.x + r.s.y, r.t.x + r.t.y};
+  a = warp_join(a, c);
   if (lane == 0) sh.warp_acc[warp] = a;
   __syncthreads();
-  if (warp == 0) a = warp_join(lane < WARPS ? sh.warp_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
+  if (warp == 0) a = warp_join(lane < WARPS ? sh.warp_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f}, c);
   if (cs > 1) {
     __syncwarp();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");       // the first CTA has started
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Pa
     __syncwarp();
     cluster.sync();
     if (rank != 0) return;
-    if (warp == 0) a = warp_join(lane < cs ? sh.cta_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f});
+    if (warp == 0) a = warp_join(lane < cs ? sh.cta_acc[lane] : Acc{-INFINITY, 0.0f, 0.0f}, c);
     if constexpr (TOP) rank_keys(top.cta_keys, cs * p.top_k, top.best);
   }
   if (warp != 0) return;
@@ -579,11 +580,11 @@ __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Pa
   if (p.stats != nullptr) {
     if (lane == 0) {
       float* s = p.stats + row * 5;
-      s[0] = a.m; s[1] = a.s; s[2] = a.t; s[3] = zt; s[4] = found ? 1.0f : 0.0f;
+      s[0] = a.m; s[1] = a.s; s[2] = a.t; s[3] = xt; s[4] = found ? 1.0f : 0.0f;
     }
     if (TOP && lane < p.top_k) p.keys[row * p.top_k + lane] = key;
   } else {
-    write_row(p, row, a, zt, found, TOP, key, lane);
+    write_row(p, row, a, xt, found, TOP, key, lane);
   }
 }
 
@@ -595,16 +596,17 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(const Params p, cons
   const long long row = blockIdx.x * 8ll + (threadIdx.x >> 5);
   if (row >= rows) return;
   Acc a{-INFINITY, 0.0f, 0.0f};
-  float zt = 0.0f;
+  const float c = p.inv_t * LOG2E;
+  float xt = 0.0f;
   bool found = false;
   u64 list = 0;
   for (int q = 0; q < parts; ++q) {
     const float* s = stats + (q * rows + row) * 5;
-    a = join(a, Acc{s[0], s[1], s[2]});
-    if (s[4] != 0.0f) { zt = s[3]; found = true; }
+    a = join(a, Acc{s[0], s[1], s[2]}, c);
+    if (s[4] != 0.0f) { xt = s[3]; found = true; }
     if (p.top_k > 0) list = warp_merge(list, lane < p.top_k ? keys[(q * rows + row) * p.top_k + lane] : 0, lane);
   }
-  write_row(p, row, a, zt, found, p.top_k > 0, list, lane);
+  write_row(p, row, a, xt, found, p.top_k > 0, list, lane);
 }
 
 struct BackParams {

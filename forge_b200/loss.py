@@ -117,7 +117,8 @@ def logprob_parts(logits, targets, vocab_start: int, vocab_total: int, top_k: in
 
 def join_logprob_parts(stats, keys, targets, vocab_total: int, temperature: float = 1.0, ignore_index: int = -100):
     """The rows' results from the parts of all slices, ``stats`` (parts, rows, 5) and ``keys`` (parts, rows, top_k):
-    ``(logprobs, entropy, lse, top_logprobs, top_ids)``, each with the rows as its first dimension."""
+    ``(logprobs, entropy, lse, top_logprobs, top_ids)``, each with the rows as its first dimension.  ``temperature`` and
+    ``ignore_index`` are those of the parts."""
     _require_cuda(stats, keys, targets)
     if keys.dim() != 3:
         raise ValueError(f"keys must be (parts, rows, top_k) (got {tuple(keys.shape)})")

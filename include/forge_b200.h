@@ -328,7 +328,7 @@ size_t forge_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t H);
  * Vocabulary slices (a row-sharded lm_head): the logits are columns [vocab_start, vocab_start + vocab) of
  * vocab_total; with `stats` non-NULL the forward writes stats (rows, 5) and keys (rows, top_k) instead of
  * results, and forge_logprobs_join turns the `parts` slices' stats (parts, rows, 5) and keys (parts, rows,
- * top_k) into the results. */
+ * top_k) into the results; its args have the temperature and the ignore_index of the slices. */
 typedef struct ForgeLogprobsArgs {
   const void* logits;
   const int64_t* targets;    /* NULL: every row is ignored (entropy and alternatives only)              */

@@ -1,0 +1,83 @@
+"""Token log probabilities where fp32 is short of room: masks of the type's lowest value at low temperatures."""
+
+import math
+
+import pytest
+import torch
+
+from forge_b200.loss import join_logprob_parts, logprob_parts, token_logprobs
+
+from tests.test_logprobs_gpu import DEV, make, reference
+
+pytestmark = pytest.mark.gpu
+
+
+def close(got, want, tol):
+    """Equal where `want`, rounded to fp32, is infinite or NaN; elsewhere within `tol` and the roundings of a number that is a
+    masked logit over the temperature (difference, reciprocal, product: 3 2^-24 of it)."""
+    w, got = want.float(), got.detach()
+    assert torch.equal(got.isnan(), w.isnan()) and torch.equal(got == -math.inf, w == -math.inf)
+    ok = w.isfinite()
+    assert ((got.double() - want).abs() <= tol + 2.0 ** -22 * want.abs())[ok].all()
+
+
+def lowest(x, dtype):
+    return torch.where(x == -math.inf, torch.finfo(dtype).min, x.float()).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [0.05, 0.7, 1.0, 1.6])
+@pytest.mark.parametrize("rows,vocab", [(5, 128256), (700, 9001)])
+def test_masks_of_the_lowest_value(dtype, temperature, rows, vocab):
+    """Nearly everything masked, so that whole threads, warps and CTAs of a row hold nothing else: the definition in 64 bits,
+    where such a logit has probability 0 too.  Tolerances as in test_logprobs_gpu.py."""
+    x, t = make(rows, vocab, dtype, masked=0.999, seed=51)
+    x[1, 1:] = -math.inf                                  # one column left
+    x[2] = -math.inf                                      # none: a uniform row
+    x[3, :vocab // 2] = -math.inf
+    x[3, -1] = 2.0
+    t[0], t[1] = 0, 0
+    low = lowest(x, dtype).requires_grad_(True)
+    out = token_logprobs(low, t, top_k=4, temperature=temperature)
+    lp, p, ent, chosen, _ = reference(low.detach(), t, temperature, -100)
+    tol = 4e-5 + 2.0 ** -22 * torch.where(x == -math.inf, 0.0, x.float()).abs().amax(-1).double() / temperature
+    close(out.logprobs, chosen, tol)
+    close(out.entropy, ent, 2 * tol)
+    ids = torch.sort(low.detach(), dim=-1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(out.top_ids, ids)
+    close(out.top_logprobs, lp.gather(-1, ids), tol[:, None].expand(-1, 4))
+    g = torch.Generator(device=DEV).manual_seed(1)
+    gl, gh = (torch.randn(rows, device=DEV, generator=g) for _ in range(2))
+    (dx,) = torch.autograd.grad((out.logprobs, out.entropy), (low,), (gl, gh))
+    gl, gh, at = gl.double()[:, None], gh.double()[:, None], t[:, None]
+    lpc = torch.where(p > 0, lp, 0.0)
+    want = (-gl * p - gh * p * (lpc + ent[:, None])).scatter_add_(-1, at, gl) / temperature
+    # d(p (log p + H)) = p (log p + H + 1) dlog p + p dH: where log p + H is next to nothing, as in a row with one column left, the
+    # errors of log p (tol) and H (2 tol) still come times p
+    terms = (gl.abs() * p + gh.abs() * p * (lpc.abs() + ent[:, None] + 1)).scatter_add_(-1, at, gl.abs()) / temperature
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + (3 * tol[:, None] + 1e-6) * terms + 1e-30
+    some = torch.arange(rows, device=DEV) != 2
+    assert ((dx.double() - want).abs() <= bound)[some].all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [0.3, 0.9])
+def test_slices_masked_with_the_lowest_value(dtype, temperature):
+    vocab, cuts = 10007, [0, 3, 4096, 10007]
+    x, t = make(11, vocab, dtype, seed=52, masked=0.99)
+    x[4, :4096] = -math.inf                               # slices with nothing else
+    x[5, 1:] = -math.inf
+    x[6] = -math.inf
+    t[4], t[5], t[7] = 10006, 0, -100
+    x[4, 10006] = 1.0
+    low = lowest(x, dtype)
+    parts = [logprob_parts(low[:, a:b], t, a, vocab, top_k=3, temperature=temperature) for a, b in zip(cuts, cuts[1:])]
+    lp, ent, lse, top, ids = join_logprob_parts(torch.stack([s for s, _ in parts]), torch.stack([k for _, k in parts]), t, vocab,
+                                                temperature=temperature)
+    want, _, want_ent, chosen, _ = reference(low, t, temperature, -100)
+    tol = 4e-5 + 2.0 ** -22 * torch.where(x == -math.inf, 0.0, x.float()).abs().amax(-1).double() / temperature
+    close(lp, chosen, tol)
+    close(ent, want_ent, 2 * tol)
+    close(lse, torch.logsumexp(low.double() / temperature, -1), 2 * tol)
+    assert torch.equal(ids, torch.sort(low, dim=-1, descending=True, stable=True).indices[:, :3])
+    close(top, want.gather(-1, ids), tol[:, None].expand(-1, 3))
