@@ -1,15 +1,17 @@
 // Log probability of one given token per row of logits, the row's entropy and its most likely
 // alternatives, and the gradient of the first two with respect to the logits.  With z = x / temperature
-// and m any number near the row's maximum, of the logits as they are:
+// and m the row's maximum, of the logits as they are:
 //   e_j = e^((x_j - m) / temperature)      S = sum e_j      T = sum (x_j - m) e_j      lse = m / temperature + log S
 //   logprob = (x_t - m) / temperature - log S      entropy = log S - T / (S temperature)      p_j = e^(z_j - lse)
 // Everything but lse is formed from differences of logits: m / temperature need not even be finite (logits of the
 // type's lowest value at a temperature below 1).
 //   dx_j = ( g_l (1[j = t] - p_j) - g_h p_j (log p_j + entropy) ) / temperature
 //
-// Forward: ONE pass over the logits.  Every thread keeps a running (m, S, T) of its own; m moves only
-// when a value exceeds it by more than LAZY_LOG, so rescaling is rare (S then stays below V e^LAZY_LOG
-// in fp32).  The partial results of threads, warps and CTAs are joined by the same rule.  A row belongs
+// Forward: ONE pass over the logits.  Every thread keeps a running (m, S, T) of its own, m the largest
+// logit so far: log S and -T / S are then both positive, and nothing cancels in the entropy of a row that is nearly
+// certain (letting m lag by up to 6, to rescale less often, left 7e-7 in it, whatever the entropy was).  A batch's
+// exponentials are added to each other before they are added to S, of which they are a small part then.
+// The partial results of threads, warps and CTAs are joined by the same rule.  A row belongs
 // to a CLUSTER of CTAs (1 for many rows, up to 16 for a few): the join over a long row goes through
 // distributed shared memory, so there is one launch, no workspace, no atomic and a fixed order -- the
 // result is bit-reproducible.
@@ -44,7 +46,6 @@ constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 16;
 constexpr int MAX_TOP = 32;
-constexpr float LAZY_LOG = 6.0f;        // e^6 = 403: far from fp32's range even times the largest vocabulary
 constexpr float LOG2E = 1.44269504088896340736f;
 
 struct Params {
@@ -175,12 +176,12 @@ __device__ __forceinline__ u64 warp_merge(u64 a, u64 b, int lane) {
 
 // ----- one thread's running sums ------------------------------------------------------------------
 struct Run {
-  float m, thr;                          // rescale when a value exceeds thr
+  float m;                               // the largest logit so far
   float nm;                              // -m, or 0 while there is no finite logit
   float2 s, t;                           // two interleaved partial sums
 };
 
-__device__ __forceinline__ void rebase(Run& r, float vmax, float lazy, float c) {
+__device__ __forceinline__ void rebase(Run& r, float vmax, float c) {
   if (r.m != -INFINITY) {
     const float d = r.m - vmax;
     const float f = exp2_approx(d * c);
@@ -192,23 +193,22 @@ __device__ __forceinline__ void rebase(Run& r, float vmax, float lazy, float c) 
   }
   r.m = vmax;
   r.nm = -vmax;
-  r.thr = vmax + lazy;
 }
 
 // adds N logits whose masked (-inf) ones have been replaced by a finite number so low that its exponential is 0 and the
 // product in T stays 0
 template <int N>
-__device__ __forceinline__ void accumulate(Run& r, float2& t, const float (&x)[N], float c) {
+__device__ __forceinline__ void accumulate(float nm, float2& s, float2& t, const float (&x)[N], float c) {
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
-    const float2 z = fadd2(make_float2(x[i], x[i + 1]), make_float2(r.nm, r.nm));
+    const float2 z = fadd2(make_float2(x[i], x[i + 1]), make_float2(nm, nm));
     const float2 y = fmul2(z, make_float2(c, c));
     const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-    r.s = fadd2(r.s, e);
+    s = fadd2(s, e);
     t = ffma2(e, z, t);
   }
 }
-// the same for logits as they are
+// the same for logits as they are, into the running sums
 template <int N>
 __device__ __forceinline__ void accumulate_raw(Run& r, const float (&x)[N], float c) {
 #pragma unroll
@@ -407,10 +407,8 @@ __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Pa
   const int v_begin = min(rank * per, nv), v_end = min(v_begin + per, nv);
 
   const float c = p.inv_t * LOG2E;
-  const float lazy = LAZY_LOG / p.inv_t;
   Run r;
   r.m = -INFINITY;
-  r.thr = -INFINITY;
   r.nm = 0.0f;
   r.s = r.t = make_float2(0.0f, 0.0f);
 
@@ -428,7 +426,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Pa
   if (warp == 0 && lane < n_one) {
     const int col = lane < head ? lane : tail0 + (lane - head);
     const float x[1] = {V::one(base + static_cast<long long>(col) * ES)};
-    if (x[0] > r.thr) rebase(r, x[0], lazy, c);
+    if (x[0] > r.m) rebase(r, x[0], c);
     accumulate_raw<1>(r, x, c);
     if constexpr (TOP) top.col[lane] = col;
   }
@@ -457,23 +455,22 @@ __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Pa
     float mx = V::max_of(q[0]);
 #pragma unroll
     for (int u = 1; u < U; ++u) mx = fmaxf(mx, V::max_of(q[u]));
-    if (mx > r.thr) rebase(r, mx, lazy, c);
-    float2 t = make_float2(0.0f, 0.0f);
-    const Run before = r;
+    if (mx > r.m) rebase(r, mx, c);
+    float2 s = make_float2(0.0f, 0.0f), t = s;
     // (a maximum as low as what stands for a masked logit: take them as they are)
     if (r.m > -1.0e38f) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float x[N];
         V::unpack(V::unmask(q[u]), x);
-        accumulate<N>(r, t, x, c);
+        accumulate<N>(r.nm, s, t, x, c);
       }
     }
     const float tt = t.x + t.y;
     if (r.m > -1.0e38f && tt == tt) {
+      r.s = fadd2(r.s, s);
       r.t = fadd2(r.t, t);
     } else {
-      r = before;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float x[N];

@@ -1,4 +1,5 @@
-"""Token log probabilities where fp32 is short of room: masks of the type's lowest value at low temperatures."""
+"""Token log probabilities where fp32 is short of room: masks of the type's lowest value at low temperatures, rows that are
+nearly certain."""
 
 import math
 
@@ -81,3 +82,23 @@ def test_slices_masked_with_the_lowest_value(dtype, temperature):
     close(lse, torch.logsumexp(low.double() / temperature, -1), 2 * tol)
     assert torch.equal(ids, torch.sort(low, dim=-1, descending=True, stable=True).indices[:, :3])
     close(top, want.gather(-1, ids), tol[:, None].expand(-1, 3))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [1.0, 0.5])
+def test_entropy_of_nearly_certain_rows(dtype, temperature):
+    """Two logits a row, the smaller one first, in columns that one thread reads one after the other; the rest masked.  With
+    g = gap / temperature, e = e^-g: S = 1 + e, H = log S + g e / S.  S is below 2 and rounded once: 2^-24.  e is off by
+    g 2^-23 (two roundings of its argument) and 2^-22 (the instruction) of itself, which H feels times g e S < H S: 2^-20 H up to
+    g = 8, and less than a hundredth of 2^-24 beyond.  The logarithm and the last sum are off by 2^-24 of H each.
+    Together: 2^-23 + 2^-20 H."""
+    rows, vocab = 700, 20008                              # one CTA per row, which reads 8192 or 4096 columns at a time
+    gaps = torch.linspace(0.25, 16.0, rows, device=DEV).to(dtype)
+    x = torch.full((rows, vocab), -math.inf, device=DEV, dtype=dtype)
+    r = torch.arange(rows, device=DEV)
+    t = r % 1024 + 8192
+    x[r, t - 8192], x[r, t] = -gaps, 0.0
+    out = token_logprobs(x, t, temperature=temperature)
+    _, _, ent, chosen, _ = reference(x, t, temperature, -100)
+    assert ((out.entropy.double() - ent).abs() <= 2.0 ** -23 + 2.0 ** -20 * ent).all()
+    assert ((out.logprobs.double() - chosen).abs() <= 2.0 ** -23 + 2.0 ** -20 * chosen.abs()).all()
