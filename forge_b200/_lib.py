@@ -135,7 +135,7 @@ class ForgeLogprobsArgs(ctypes.Structure):
                 ("ignore_index", ctypes.c_int64), ("temperature", ctypes.c_double), ("dtype", ctypes.c_int32),
                 ("top_k", ctypes.c_int32), ("logprobs", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("lse", ctypes.c_void_p),
                 ("top_logprobs", ctypes.c_void_p), ("top_ids", ctypes.c_void_p), ("stats", ctypes.c_void_p),
-                ("keys", ctypes.c_void_p)]
+                ("keys", ctypes.c_void_p), ("row_max", ctypes.c_void_p), ("log_sum", ctypes.c_void_p)]
 
 
 class ForgeMultiItem(ctypes.Structure):

@@ -4,7 +4,8 @@
 //   e_j = e^((x_j - m) / temperature)      S = sum e_j      T = sum (x_j - m) e_j      lse = m / temperature + log S
 //   logprob = (x_t - m) / temperature - log S      entropy = log S - T / (S temperature)      p_j = e^(z_j - lse)
 // Everything but lse is formed from differences of logits: m / temperature need not even be finite (logits of the
-// type's lowest value at a temperature below 1).
+// type's lowest value at a temperature below 1), and a constant added to a row changes nothing.  The gradient, too: from lse
+// alone, log p_j would have lse's rounding, 8 % of a gradient at logits near 1000 and a temperature of 0.7.
 //   dx_j = ( g_l (1[j = t] - p_j) - g_h p_j (log p_j + entropy) ) / temperature
 //
 // Forward: ONE pass over the logits.  Every thread keeps a running (m, S, T) of its own, m the largest
@@ -56,6 +57,8 @@ struct Params {
   float* lse;
   float* top_logprobs;
   long long* top_ids;
+  float* row_max;
+  float* log_sum;
   float* stats;                          // partial mode: (rows, 5) = m, S, T, target's logit, target found
   unsigned long long* keys;              // partial mode: (rows, top_k)
   long long vocab, ld, ignore_index, vocab_start, vocab_total;
@@ -338,6 +341,8 @@ __device__ __forceinline__ void write_row(const Params& p, long long row, const 
     if (p.logprobs) p.logprobs[row] = ignored ? 0.0f : (found ? (xt - a.m) * p.inv_t - log_s : NAN);
     if (p.entropy) p.entropy[row] = log_s - a.t / a.s * p.inv_t;
     if (p.lse) p.lse[row] = a.m * p.inv_t + log_s;
+    if (p.row_max) p.row_max[row] = a.m;
+    if (p.log_sum) p.log_sum[row] = log_s;
   }
   if (top && lane < p.top_k) {
     // fewer than k comparable logits (NaN): any valid column
@@ -610,7 +615,8 @@ struct BackParams {
   const uint8_t* logits;
   uint8_t* grad;
   const long long* targets;
-  const float* lse;
+  const float* row_max;                  // or NULL, and log_sum is lse
+  const float* log_sum;
   const float* entropy;
   const float* g_logprob;
   const float* g_entropy;
@@ -658,7 +664,8 @@ __global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const B
                    : (t < 0 || t >= p.vocab_total)     ? NAN
                                                        : p.g_logprob[row] * p.inv_t;
   const float c = p.inv_t * LOG2E;
-  const float nl = -p.lse[row] * LOG2E;                  // log2 p = x c + nl
+  const float m = p.row_max ? p.row_max[row] : 0.0f;
+  const float nl = -p.log_sum[row] * LOG2E;              // log2 p = (x - m) c + nl
   const float gh = ENT ? p.g_entropy[row] * p.inv_t : 0.0f;
   // dx = p (-gl - gh (log p + H)) + gl [j = t] = p (a + b log2 p) + ...
   const float a = ENT ? -gl - gh * p.entropy[row] : -gl;
@@ -666,7 +673,7 @@ __global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const B
   const long long tl = t - p.vocab_start;                // column of the target, if it is one of these
   const bool here = !ignored && tl >= 0 && tl < p.vocab;
   auto one = [&](float x) {
-    const float y = __fmaf_rn(x, c, nl);
+    const float y = __fmaf_rn(x - m, c, nl);
     const float pr = exp2_approx(y);
     // (below -127 the probability is 0, and its logarithm must stay finite whatever b is)
     if constexpr (ENT) return pr * __fmaf_rn(b, max_nan(y, -127.0f), a);
@@ -750,7 +757,7 @@ static int check(const ForgeLogprobsArgs& a, const char* what) {
   if (a.rows * MAX_CLUSTER > 0x7fffffffll) return fail(FORGE_ERR_SHAPE, "%s: %lld rows", what, (long long)a.rows);
   auto off = [](const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
   if (off(a.targets, 8) || off(a.logprobs, 4) || off(a.entropy, 4) || off(a.lse, 4) || off(a.top_logprobs, 4) || off(a.top_ids, 8) ||
-      off(a.stats, 4) || off(a.keys, 8))
+      off(a.stats, 4) || off(a.keys, 8) || off(a.row_max, 4) || off(a.log_sum, 4))
     return fail(FORGE_ERR_ALIGNMENT, "%s: targets or outputs are not element-aligned", what);
   return FORGE_OK;
 }
@@ -760,6 +767,7 @@ static Params make_params(const ForgeLogprobsArgs& a) {
   p.logits = static_cast<const uint8_t*>(a.logits);
   p.targets = reinterpret_cast<const long long*>(a.targets);
   p.logprobs = a.logprobs; p.entropy = a.entropy; p.lse = a.lse;
+  p.row_max = a.row_max; p.log_sum = a.log_sum;
   p.top_logprobs = a.top_logprobs; p.top_ids = reinterpret_cast<long long*>(a.top_ids);
   p.stats = a.stats; p.keys = reinterpret_cast<u64*>(a.keys);
   p.vocab = a.vocab; p.ld = a.ld; p.ignore_index = a.ignore_index;
@@ -861,7 +869,8 @@ extern "C" int forge_logprobs_backward(const ForgeLogprobsArgs* args, const floa
   int rc = loss::check(a, "forge_logprobs_backward");
   if (rc != FORGE_OK) return rc;
   if (a.rows == 0) return FORGE_OK;
-  if (a.logits == nullptr || a.lse == nullptr || grad == nullptr || (g_entropy != nullptr && a.entropy == nullptr))
+  const bool apart = a.row_max != nullptr && a.log_sum != nullptr;
+  if (a.logits == nullptr || (!apart && a.lse == nullptr) || grad == nullptr || (g_entropy != nullptr && a.entropy == nullptr))
     return fail(FORGE_ERR_INVALID_ARG, "forge_logprobs_backward: null pointer");
   if (ld_grad < a.vocab) return fail(FORGE_ERR_SHAPE, "forge_logprobs_backward: ld_grad=%lld", (long long)ld_grad);
   const int es = a.dtype == FORGE_DT_BF16 ? 2 : 4;
@@ -872,7 +881,8 @@ extern "C" int forge_logprobs_backward(const ForgeLogprobsArgs* args, const floa
   p.logits = static_cast<const uint8_t*>(a.logits);
   p.grad = static_cast<uint8_t*>(grad);
   p.targets = reinterpret_cast<const long long*>(a.targets);
-  p.lse = a.lse; p.entropy = a.entropy; p.g_logprob = g_logprob; p.g_entropy = g_entropy;
+  p.row_max = apart ? a.row_max : nullptr; p.log_sum = apart ? a.log_sum : a.lse;
+  p.entropy = a.entropy; p.g_logprob = g_logprob; p.g_entropy = g_entropy;
   p.vocab = a.vocab; p.ld = a.ld; p.ld_grad = ld_grad; p.ignore_index = a.ignore_index;
   p.vocab_start = a.vocab_start; p.vocab_total = a.vocab_total;
   p.inv_t = static_cast<float>(1.0 / a.temperature);

@@ -74,27 +74,29 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& l
   return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
 }
 
-// {logprobs, entropy, lse (if it is wanted), top_logprobs, top_ids}
-std::array<at::Tensor, 5> loss_forward(const at::Tensor& x, const at::Tensor& t, int64_t top_k, double temperature, int64_t ignore,
-                                       bool with_lse) {
+// {logprobs, entropy, top_logprobs, top_ids, and for the gradient row_max, log_sum}
+std::array<at::Tensor, 6> loss_forward(const at::Tensor& x, const at::Tensor& t, int64_t top_k, double temperature, int64_t ignore,
+                                       bool gradient) {
   Rows r;
   as_rows(x, r);
   const int dev = x.get_device();
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
   ForgeLogprobsArgs a = loss_args(x, r, t, top_k, temperature, ignore);
   const auto lead = x.sizes().slice(0, x.dim() - 1);
-  std::array<at::Tensor, 5> out;
-  for (int i = 0; i < (with_lse ? 3 : 2); ++i) out[i] = empty(lead, at::kFloat, x);
-  a.logprobs = static_cast<float*>(out[0].data_ptr());
-  a.entropy = static_cast<float*>(out[1].data_ptr());
-  a.lse = with_lse ? static_cast<float*>(out[2].data_ptr()) : nullptr;
+  std::array<at::Tensor, 6> out;
+  float** const per_row[6] = {&a.logprobs, &a.entropy, nullptr, nullptr, &a.row_max, &a.log_sum};
+  for (int i : {0, 1, 4, 5}) {
+    if (i >= 4 && !gradient) continue;
+    out[i] = empty(lead, at::kFloat, x);
+    *per_row[i] = static_cast<float*>(out[i].data_ptr());
+  }
   if (top_k > 0) {
     c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end());
     shape.push_back(top_k);
-    out[3] = empty(shape, at::kFloat, x);
-    out[4] = empty(shape, at::kLong, x);
-    a.top_logprobs = static_cast<float*>(out[3].data_ptr());
-    a.top_ids = static_cast<int64_t*>(out[4].data_ptr());
+    out[2] = empty(shape, at::kFloat, x);
+    out[3] = empty(shape, at::kLong, x);
+    a.top_logprobs = static_cast<float*>(out[2].data_ptr());
+    a.top_ids = static_cast<int64_t*>(out[3].data_ptr());
   }
   check(forge_logprobs_forward(&a, stream_of(dev)), "forge_logprobs_forward");
   return out;
@@ -105,13 +107,13 @@ class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& t, int64_t top_k, double temperature,
                                int64_t ignore) {
     auto out = loss_forward(x, t, top_k, temperature, ignore, true);
-    ctx->save_for_backward({x, t, out[2], out[1]});
+    ctx->save_for_backward({x, t, out[1], out[4], out[5]});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore"] = ignore;
     ctx->set_materialize_grads(false);
     if (top_k > 0) {
-      ctx->mark_non_differentiable({out[3], out[4]});
-      return {out[0], out[1], out[3], out[4]};
+      ctx->mark_non_differentiable({out[2], out[3]});
+      return {out[0], out[1], out[2], out[3]};
     }
     return {out[0], out[1]};
   }
@@ -131,8 +133,8 @@ class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
       const int dev = x.get_device();
       c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
       ForgeLogprobsArgs a = loss_args(x, r, t, 0, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt());
-      a.lse = static_cast<float*>(const_cast<void*>(saved[2].const_data_ptr()));
-      a.entropy = static_cast<float*>(const_cast<void*>(saved[3].const_data_ptr()));
+      float** const per_row[3] = {&a.entropy, &a.row_max, &a.log_sum};
+      for (int i = 0; i < 3; ++i) *per_row[i] = static_cast<float*>(const_cast<void*>(saved[2 + i].const_data_ptr()));
       dx = empty(x.sizes(), x.scalar_type(), x);
       check(forge_logprobs_backward(&a, gr[0].defined() ? static_cast<const float*>(gr[0].const_data_ptr()) : nullptr,
                                     gr[1].defined() ? static_cast<const float*>(gr[1].const_data_ptr()) : nullptr, dx.data_ptr(), r.vocab,
@@ -161,7 +163,7 @@ py::object token_logprobs(const at::Tensor& x, const c10::optional<at::Tensor>& 
     return py::make_tuple(wrap(out[0]), wrap(out[1]), top_k ? wrap(out[2]) : none, top_k ? wrap(out[3]) : none);
   }
   const auto out = loss_forward(x, t, top_k, temperature, ignore, false);
-  return py::make_tuple(wrap(out[0]), wrap(out[1]), top_k ? wrap(out[3]) : none, top_k ? wrap(out[4]) : none);
+  return py::make_tuple(wrap(out[0]), wrap(out[1]), top_k ? wrap(out[2]) : none, top_k ? wrap(out[3]) : none);
 }
 
 // ----- AdamW over a list of tensors -----------------------------------------------------------------

@@ -89,16 +89,21 @@ def _call(fn, device, *args):
         _lib.check(rc, fn)
 
 
-def _outputs(a, lead, top_k, device):
+_SAVED = ("row_max", "log_sum")      # what backward needs besides the entropy
+
+
+def _outputs(a, lead, top_k, device, more):
+    """``(logprobs, entropy, top_logprobs, top_ids, *more)``, `more` naming other outputs of a value per row."""
     # (tensors of their own and no views: what a user does in place to one result is not done to the saved ones)
-    out = [torch.empty(lead, dtype=torch.float32, device=device) for _ in range(3)]
-    a.logprobs, a.entropy, a.lse = (t.data_ptr() for t in out)
+    out = [torch.empty(lead, dtype=torch.float32, device=device) for _ in range(2 + len(more))]
+    for name, t in zip(("logprobs", "entropy", *more), out):
+        setattr(a, name, t.data_ptr())
     top = ids = None
     if top_k:
         top = torch.empty(*lead, top_k, dtype=torch.float32, device=device)
         ids = torch.empty(*lead, top_k, dtype=torch.int64, device=device)
         a.top_logprobs, a.top_ids = top.data_ptr(), ids.data_ptr()
-    return out[0], out[1], out[2], top, ids
+    return out[0], out[1], top, ids, *out[2:]
 
 
 def logprob_parts(logits, targets, vocab_start: int, vocab_total: int, top_k: int = 0, temperature: float = 1.0,
@@ -132,16 +137,17 @@ def join_logprob_parts(stats, keys, targets, vocab_total: int, temperature: floa
                          f"{tuple(keys.shape)})")
     if t is not None and t.numel() != rows:
         raise ValueError(f"{t.numel()} targets for {rows} rows")
-    return _join(stats, keys, t, vocab_total, temperature, ignore_index, (rows,))
+    lp, ent, top, ids, lse = _join(stats, keys, t, vocab_total, temperature, ignore_index, (rows,), ("lse",))
+    return lp, ent, lse, top, ids
 
 
-def _join(stats, keys, t, vocab_total, temperature, ignore_index, lead):
+def _join(stats, keys, t, vocab_total, temperature, ignore_index, lead, more):
     parts, rows, top_k = keys.shape
     a = _lib.ForgeLogprobsArgs()
     a.targets = t.data_ptr() if t is not None else None
     a.rows, a.vocab_total, a.vocab, a.ld = rows, vocab_total, vocab_total, vocab_total
     a.ignore_index, a.temperature, a.top_k = ignore_index, temperature, top_k
-    res = _outputs(a, lead, top_k, stats.device)
+    res = _outputs(a, lead, top_k, stats.device, more)
     _call("forge_logprobs_join", stats.device, ctypes.byref(a), stats.data_ptr(), keys.data_ptr(), parts)
     return res
 
@@ -167,16 +173,17 @@ class _TokenLogprobs(torch.autograd.Function):
         lead = logits.shape[:-1]
         if group is None:
             a = _args(x, t, top_k, temperature, ignore_index, vocab_start, vocab_total)
-            lp, ent, lse, top, ids = _outputs(a, lead, top_k, x.device)
+            lp, ent, top, ids, *saved = _outputs(a, lead, top_k, x.device, _SAVED)
             _call("forge_logprobs_forward", x.device, ctypes.byref(a))
         else:
             stats, keys = logprob_parts(x, t, vocab_start, vocab_total, top_k, temperature, ignore_index)
-            lp, ent, lse, top, ids = _join(*_gather_parts(stats, keys, group), t, vocab_total, temperature, ignore_index, lead)
+            lp, ent, top, ids, *saved = _join(*_gather_parts(stats, keys, group), t, vocab_total, temperature, ignore_index, lead,
+                                              _SAVED)
         if top_k:
             ctx.mark_non_differentiable(top, ids)
         ctx.set_materialize_grads(False)
         # the logits themselves where they are rows already, so that autograd notices if they are changed
-        ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, t, lse, ent)
+        ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, t, ent, *saved)
         ctx.shape = logits.shape
         ctx.settings = (temperature, ignore_index, vocab_start, vocab_total)
         return lp, ent, top, ids
@@ -184,13 +191,14 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_ent, _g_top, _g_ids):
-        x, t, lse, ent = ctx.saved_tensors
+        x, t, *saved = ctx.saved_tensors
         x = _rows(x)
         none = (None,) * 7
         if g_lp is None and g_ent is None:
             return (None, *none)
         a = _args(x, t, 0, *ctx.settings)
-        a.entropy, a.lse = ent.data_ptr(), lse.data_ptr()
+        for name, s in zip(("entropy", *_SAVED), saved):
+            setattr(a, name, s.data_ptr())
         g = [None if q is None else q.reshape(-1).to(torch.float32).contiguous() for q in (g_lp, g_ent)]
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         _call("forge_logprobs_backward", x.device, ctypes.byref(a), *(None if q is None else q.data_ptr() for q in g),

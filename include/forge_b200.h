@@ -320,6 +320,7 @@ size_t forge_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t H);
  *   logprobs[r] = z[t] - log sum_j e^z[j] for the given token t = targets[r]; 0 where t == ignore_index, NaN
  *                 where t is outside [0, vocab_total) (nothing is read there)
  *   entropy[r]  = -sum_j p_j log p_j,   lse[r] = log sum_j e^z[j]
+ *   row_max[r]  = the largest logit x (of the whole vocabulary), log_sum[r] = log sum_j e^((x[j] - row_max) / temperature)
  *   top_logprobs / top_ids (rows, top_k): the top_k <= 32 largest logits' log probabilities and columns, in
  *                 descending order, equal logits by ascending column
  * A logit of -inf has probability zero; a row of nothing else, or with a NaN or +inf, gives NaN as the
@@ -345,14 +346,17 @@ typedef struct ForgeLogprobsArgs {
   int64_t* top_ids;
   float* stats;
   uint64_t* keys;
+  float* row_max;            /* (rows,)                                                                 */
+  float* log_sum;            /* (rows,)                                                                 */
 } ForgeLogprobsArgs;
 int forge_logprobs_forward(const ForgeLogprobsArgs* args, void* cuda_stream);
 int forge_logprobs_join(const ForgeLogprobsArgs* args, const float* stats, const uint64_t* keys, int32_t parts,
                         void* cuda_stream);
 
 /* grad[r, j] = (g_logprob[r] (1[j = t] - p_j) - g_entropy[r] p_j (log p_j + entropy[r])) / temperature, in the
- * logits' type, row pitch ld_grad.  args: as in the forward, with `lse` (and `entropy`, if g_entropy is given)
- * as it wrote them; the logits of a slice give the slice's columns of the gradient.  g_logprob, g_entropy:
+ * logits' type, row pitch ld_grad.  args: as in the forward, with `row_max` and `log_sum` (and `entropy`, if g_entropy is
+ * given) as it wrote them, or, without those two, with `lse`: p_j then has the rounding of lse, 2^-24 of its size, where
+ * the former only has that of x_j - row_max.  The logits of a slice give the slice's columns of the gradient.  g_logprob, g_entropy:
  * (rows,) or NULL for zero.  A row for which both are zero (or the target is ignored and the second is) gets zeros,
  * whatever its logits are. */
 int forge_logprobs_backward(const ForgeLogprobsArgs* args, const float* g_logprob, const float* g_entropy, void* grad,

@@ -102,3 +102,91 @@ def test_entropy_of_nearly_certain_rows(dtype, temperature):
     _, _, ent, chosen, _ = reference(x, t, temperature, -100)
     assert ((out.entropy.double() - ent).abs() <= 2.0 ** -23 + 2.0 ** -20 * ent).all()
     assert ((out.logprobs.double() - chosen).abs() <= 2.0 ** -23 + 2.0 ** -20 * chosen.abs()).all()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+@pytest.mark.parametrize("offset", [50.0, -200.0, 1000.0])
+@pytest.mark.parametrize("rows", [3, 700])
+def test_a_constant_added_to_a_row_changes_nothing(rows, offset, temperature):
+    """Logits on a grid of 2^-10, so that adding the constant is exact, and so is every difference of two: the same bits, by
+    the direct call and, for rows of a wider pitch, by the Python one."""
+    vocab = 32003
+    g = torch.Generator(device=DEV).manual_seed(53)
+    x = ((torch.randn(rows, vocab, device=DEV, generator=g) * 2.5).clamp(-16, 16) * 1024).round() / 1024
+    t = torch.randint(0, vocab, (rows,), device=DEV, generator=g)
+    x[torch.arange(rows, device=DEV), t] = 14.0
+    gl, gh = (torch.randn(rows, device=DEV, generator=g) for _ in range(2))
+
+    def results(x, three_dimensional):
+        x = x.requires_grad_(True)
+        if three_dimensional:
+            v, tt = torch.cat([x, x.detach()], 1)[:, :vocab][None], t[None]
+        else:
+            v, tt = x, t
+        out = token_logprobs(v, tt, top_k=3, temperature=temperature)
+        (one,) = torch.autograd.grad(out.logprobs, x, gl.view_as(tt), retain_graph=True)
+        (both,) = torch.autograd.grad((out.logprobs, out.entropy), x, (gl.view_as(tt), gh.view_as(tt)))
+        return [r.reshape(rows, -1) for r in (*out, one, both)]
+
+    for nd in (False, True):
+        first, shifted = results(x.clone(), nd), results(x + offset, nd)
+        for a, b in zip(first, shifted):
+            assert torch.equal(a, b)
+
+
+def test_a_constant_added_to_sliced_rows_changes_nothing():
+    """As above for slices of the vocabulary: the joined base and sum give each slice its gradient."""
+    import ctypes
+
+    from forge_b200.loss import _SAVED, _args, _call, _join
+    vocab, cuts, rows, temperature = 5000, [0, 3, 2048, 5000], 9, 0.7
+    g = torch.Generator(device=DEV).manual_seed(54)
+    x = (torch.randn(rows, vocab, device=DEV, generator=g) * 2.5 * 1024).round() / 1024
+    t = torch.randint(0, vocab, (rows,), device=DEV, generator=g)
+    gl, gh = (torch.randn(rows, device=DEV, generator=g) for _ in range(2))
+
+    def results(x):
+        parts = [logprob_parts(x[:, a:b], t, a, vocab, temperature=temperature) for a, b in zip(cuts, cuts[1:])]
+        lp, ent, _, _, top, total = _join(torch.stack([s for s, _ in parts]), torch.stack([k for _, k in parts]), t, vocab, temperature,
+                                          -100, (rows,), _SAVED)
+        assert torch.equal(top, x.amax(1))
+        grads = []
+        for a, b in zip(cuts, cuts[1:]):
+            args = _args(x[:, a:b], t, 0, temperature, -100, a, vocab)
+            args.entropy, args.row_max, args.log_sum = ent.data_ptr(), top.data_ptr(), total.data_ptr()
+            grads.append(torch.empty(rows, b - a, device=DEV))
+            _call("forge_logprobs_backward", x.device, ctypes.byref(args), gl.data_ptr(), gh.data_ptr(), grads[-1].data_ptr(), b - a)
+        return lp, ent, total, torch.cat(grads, 1)
+
+    first, shifted = results(x), results(x + 1000.0)
+    for a, b in zip(first, shifted):
+        assert torch.equal(a, b)
+    xr = x.clone().requires_grad_(True)
+    out = token_logprobs(xr, t, temperature=temperature)
+    (want,) = torch.autograd.grad((out.logprobs, out.entropy), (xr,), (gl, gh))
+    # other orders of the same fp32 sums: 4e-5 of p, as in test_logprobs_gpu.py, and 2^-20 for what is formed of it
+    p = torch.softmax(x.double() / temperature, 1)
+    terms = (gl.abs()[:, None] + gh.abs()[:, None] * ((-p.clamp(min=1e-300).log()) + out.entropy.detach()[:, None] + 1)) * p / temperature
+    terms.scatter_add_(1, t[:, None], gl.abs().double()[:, None] / temperature)
+    assert ((first[3] - want).abs() <= (4 * 4e-5 + 2.0 ** -20) * terms).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [0.05, 0.7, 1.0])
+def test_gradient_of_a_row_of_the_lowest_value(dtype, temperature):
+    """All logits equal: a uniform row, whatever their value.  Powers of two, so p = 1 / V is exact; log p and the entropy are off
+    by 2^-22 of themselves at most, and cancel in the entropy's gradient."""
+    vocab = 4096
+    x = torch.full((2, vocab), torch.finfo(dtype).min, device=DEV, dtype=dtype, requires_grad=True)
+    t = torch.tensor([5, 4000], device=DEV)
+    out = token_logprobs(x, t, temperature=temperature)
+    log_v = math.log(vocab)
+    assert ((out.logprobs.double() + log_v).abs() <= 2.0 ** -22 * log_v).all()
+    assert ((out.entropy.double() - log_v).abs() <= 2.0 ** -22 * log_v).all()
+    (dx,) = torch.autograd.grad(out.logprobs.sum(), x, retain_graph=True)
+    want = torch.full((2, vocab), -1.0 / vocab, device=DEV, dtype=torch.float64).scatter_add_(1, t[:, None], torch.ones(2, 1, device=DEV).double())
+    want /= temperature
+    # 2^-21: of the exponent -12, of its power, of the temperature's reciprocal
+    assert ((dx.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 12 * 2.0 ** -22 + 2.0 ** -22) * want.abs() + 2.0 ** -23 / temperature / vocab).all()
+    (dx,) = torch.autograd.grad(out.entropy.sum(), x)
+    assert (dx.double().abs() <= 2 * 2.0 ** -21 * log_v / vocab / temperature).all()

@@ -212,3 +212,12 @@ def test_parts_are_gathered_in_rank_order():
     for p in procs:
         p.join(60)
     assert got == {0: "ok", 1: "ok"}, got
+
+
+def test_logprobs_row_maxima_and_sums_are_checked():
+    lib = _lib.load()
+    for kw, code in ((dict(lse=None, row_max=P), _lib.FORGE_ERR_INVALID_ARG), (dict(lse=None, log_sum=P), _lib.FORGE_ERR_INVALID_ARG),
+                     (dict(row_max=P + 2, log_sum=P), _lib.FORGE_ERR_ALIGNMENT), (dict(row_max=P, log_sum=P + 1), _lib.FORGE_ERR_ALIGNMENT)):
+        assert lib.forge_logprobs_backward(ctypes.byref(logprobs(**kw)), P, P, P, 100, None) == code
+    assert lib.forge_logprobs_forward(ctypes.byref(logprobs(row_max=P + 2)), None) == _lib.FORGE_ERR_ALIGNMENT
+    assert lib.forge_logprobs_join(ctypes.byref(logprobs(log_sum=P + 2)), P, P, 2, None) == _lib.FORGE_ERR_ALIGNMENT
