@@ -1,13 +1,15 @@
 // Direct calls of the loss, multi-tensor and 8-bit entry points of the C ABI from PyTorch, for calls that are so short
 // that marshalling them in Python would take longer than the kernels run (a decoding step's log probabilities, the
 // norm weights of a decoder).  Every function returns None for arguments that are not of the plain form it handles
-// (another dtype or layout, a wrong shape, CPU tensors); the Python wrappers then take over, which check, copy or refuse.
+// (another dtype or layout, a wrong shape, CPU tensors, a derivative carried forward or a trace being recorded); the Python
+// wrappers then take over, which check, copy or refuse.
 // Both paths issue the same library calls.
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -31,6 +33,9 @@ void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(static_cast<c1
 
 bool float_type(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
 int dtype_id(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? FORGE_DT_BF16 : FORGE_DT_F32; }
+
+// whether something besides x.requires_grad() follows what happens to x (forge_b200.native.followed)
+bool followed(const at::Tensor& x) { return torch::jit::tracer::isTracing() || x._fw_grad(0).defined(); }
 
 // an error for whoever differentiates a gradient again
 at::Tensor once(const at::Tensor& g) {
@@ -148,7 +153,7 @@ class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
 
 py::object token_logprobs(const at::Tensor& x, const c10::optional<at::Tensor>& targets, int64_t top_k, double temperature, int64_t ignore) {
   Rows r;
-  if (!as_rows(x, r) || top_k < 0 || top_k > 32 || top_k > r.vocab) return py::none();
+  if (!as_rows(x, r) || top_k < 0 || top_k > 32 || top_k > r.vocab || followed(x)) return py::none();
   at::Tensor t;
   if (targets.has_value() && targets->defined()) {
     t = *targets;
@@ -385,7 +390,7 @@ class Fp8LinearFn : public torch::autograd::Function<Fp8LinearFn> {
 
 py::object fp8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ws, const c10::optional<at::Tensor>& wt,
                       const c10::optional<at::Tensor>& wts) {
-  if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || !x.is_contiguous() || x.dim() < 1 || x.numel() == 0) return py::none();
+  if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || !x.is_contiguous() || x.dim() < 1 || x.numel() == 0 || followed(x)) return py::none();
   const int dev = x.get_device();
   if (dev >= 64 || g_status[dev] == nullptr || !code_matrix(w, dev) || x.size(-1) != w.size(1) ||
       !scale_matrix(ws, dev, blocks(w.size(0)), blocks(w.size(1))))
@@ -405,7 +410,7 @@ py::object fp8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor
 // (codes, scales[, codes of the transpose, its scales])
 py::object quantize(const at::Tensor& x, int64_t block_rows, bool transposed) {
   if (!x.is_cuda() || !float_type(x) || x.dim() != 2 || x.numel() == 0 || !x.is_contiguous() || (block_rows != 1 && block_rows != 128) ||
-      (transposed && block_rows == 1))
+      (transposed && block_rows == 1) || torch::jit::tracer::isTracing())
     return py::none();
   const int dev = x.get_device();
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));

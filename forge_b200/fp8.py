@@ -42,17 +42,23 @@ def _pitch(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), -(-t.shape[1] // 16) * 16)
 
 
+def _no_trace(what):
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced: its result would be a constant of the trace")
+
+
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1, transposed: bool = False, out=None):
     """e4m3 codes and fp32 scales of a bf16 or fp32 matrix ``x`` (R, C) in blocks of ``block_rows`` x 128 (1 or 128):
     ``scale = absmax * (1 / 448) + 1e-12``, ``code = e4m3(x / scale)`` in fp32.  Returns ``(codes (R, C), scales (ceil(R / block_rows),
     ceil(C / 128)))``; with ``transposed`` (128 x 128 blocks) also the codes (C, R) and scales of the transpose.  Code rows
-    start on 16-byte boundaries.  An infinity makes its block NaN, a NaN only itself.  ``out``: tensors of an earlier call
-    to write to."""
+    start on 16-byte boundaries.  An infinity makes its block NaN, a NaN only itself.  Codes carry no gradient.  ``out``: tensors
+    of an earlier call to write to."""
     nat = native.module() if out is None else None
     if nat is not None:
         res = nat.fp8_quantize(x, block_rows, transposed)
         if res is not None:
             return res
+    _no_trace("quantize_fp8")
     _require_cuda(x)
     _matrix(x, "x")
     if block_rows not in (1, BLOCK):
@@ -94,6 +100,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1, transposed: bool = False,
 def fp8_matmul(x_codes, x_scales, w_codes, w_scales) -> torch.Tensor:
     """``Y = X W^T`` (M, N) bf16 of codes with scales: X (M, K) with scales (M, ceil(K / 128)), W (N, K) with scales
     (ceil(N / 128), ceil(K / 128)).  Code rows start on 16-byte boundaries (those of ``quantize_fp8`` do)."""
+    _no_trace("fp8_matmul")
     _require_cuda(x_codes, x_scales, w_codes, w_scales)
     for t, what in ((x_codes, "x_codes"), (w_codes, "w_codes"), (x_scales, "x_scales"), (w_scales, "w_scales")):
         _matrix(t, what)
@@ -191,12 +198,13 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Weight, bias: torch.Tensor | None = N
             y = nat.fp8_linear(x, weight.codes, weight.scales, weight.codes_t, weight.scales_t)
         if y is not None:
             return y
+    _no_trace("fp8_linear")
     _require_cuda(x, bias)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"fp8_linear takes bfloat16 activations (got {x.dtype})")
     if x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] == 0:
         raise ValueError(f"x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
-    if not torch.is_grad_enabled() or not (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if not (torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))) and not native.followed(x, bias):
         return _forward(x, bias, weight)
     if x.requires_grad and weight.codes_t is None:
         raise ValueError("the input gradient needs the weight's transposed codes (Fp8Weight.from_weight(w, transposed=True))")

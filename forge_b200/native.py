@@ -16,6 +16,9 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+from torch.autograd import forward_ad
+
 _mod = None
 _tried = False
 
@@ -35,6 +38,13 @@ def module():
             except ImportError:
                 _mod = None
     return _mod
+
+
+def followed(*tensors) -> bool:
+    """Whether what happens to one of the tensors (or None) is recorded by other means than its ``requires_grad``: a derivative
+    that is carried forward, or a trace.  An operator then has to go through its autograd function, which refuses the first and
+    is part of the second, or refuse; the extension's direct calls leave such arguments alone."""
+    return torch.jit.is_tracing() or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def reset():
