@@ -60,7 +60,8 @@ class FusedLinearFunction(torch.autograd.Function):
         ctx.l2_manager = l2_manager
         ctx.use_fused_backward = use_fused_backward
         if fp8_products:
-            return fp8_linear(input.detach(), w8, bias)
+            # (an fp32 bias would make the output fp32, and with it the gradient that meets the bf16 input in backward)
+            return fp8_linear(input.detach(), w8, bias).to(input.dtype)
         return F.linear(input, weight, bias)
 
     @staticmethod
@@ -96,7 +97,9 @@ class FusedLinearFunction(torch.autograd.Function):
             else:
                 _apply_fused(dy2d, x2d, weight, state, config, ctx.l2_manager)
 
-        grad_bias = dy2d.sum(0) if bias is not None else None
+        grad_bias = None
+        if bias is not None:
+            grad_bias = dy2d.sum(0, dtype=bias.dtype if ctx.fp8_weight is not None else None)
         return grad_input, grad_weight, grad_bias, None, None, None, None, None, None, None
 
 

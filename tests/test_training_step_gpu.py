@@ -274,3 +274,44 @@ def test_sharded_loss_of_one_rank_equals_the_torch_ops():
         assert ((ga.double() - gb.double()).abs() <= 2.0 ** -7 * ga.double().abs() + 1e-9).all()
     finally:
         dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_fp8_products_of_an_fp32_linear(bias):
+    """fp32 weight and bias, bf16 activations: the output is bf16 as the activations are (the bias added in fp32, one
+    rounding), the weight's gradient and update come from the bf16 operands."""
+    torch.manual_seed(5)
+    lin = FusedLinear(272, 392, bias=bias).to(DEV).train().use_fp8_products()
+    x = torch.randn(37, 272, device=DEV).bfloat16().requires_grad_(True)
+    dy = (torch.randn(37, 392, device=DEV) * 0.1).bfloat16()
+    w0 = lin.weight.detach().clone()
+    y = lin(x)
+    assert y.dtype == torch.bfloat16
+    product = fp8_linear(x.detach(), Fp8Weight.from_weight(w0))
+    assert torch.equal(y, product if not bias else (product.float() + lin.bias).bfloat16())
+    y.backward(dy)
+    xr = x.detach().clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(fp8_linear(xr, Fp8Weight.from_weight(w0)), xr, dy)
+    assert torch.equal(x.grad, dx)
+    want = dy.double().t() @ x.detach().double()
+    # a sum of 37 exact products in fp32, rounded to bf16 at most
+    assert lin.weight.grad.dtype == torch.float32
+    bound = 2.0 ** -8 * want.abs() + 37 * 2.0 ** -24 * (dy.double().abs().t() @ x.detach().double().abs())
+    assert ((lin.weight.grad.double() - want).abs() <= bound).all()
+    if bias:
+        want = dy.double().sum(0)
+        assert lin.bias.grad.dtype == torch.float32
+        assert ((lin.bias.grad.double() - want).abs() <= 37 * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+    # the update, fused and with the gradient accumulated before it
+    lin.weight.grad = x.grad = None
+    lin.update_optimizer_config(OptimizerConfig(lr=1e-2))
+    lin(x).backward(dy)
+    w1, m, v = w0.clone(), torch.zeros_like(w0), torch.zeros_like(w0)
+    st = lin._state
+    K.fused_grad_adamw(dy, x.detach(), w1, m.to(st.m.dtype), v.to(st.v.dtype), lr=1e-2, step=1)
+    assert torch.equal(lin.weight, w1) and not torch.equal(w1, w0) and torch.equal(x.grad, dx)
+    lin.set_accumulating(True)
+    lin(x).backward(dy)
+    lin.set_accumulating(False)
+    lin(x).backward(dy)
+    assert lin.weight.isfinite().all() and not torch.equal(lin.weight, w1)
