@@ -329,6 +329,25 @@ __device__ __forceinline__ double block_sum_d(double v, double* red) {
   return t;
 }
 
+// The sum of eight squares: in fp32, or, where that has left its range (a square above 3.4e38 or all of them so small that
+// what is lost below 2^-149 would be missed), in fp64.  Zeros, of which an embedding's gradient mostly consists, are told apart
+// before they are converted.
+__device__ __forceinline__ double sum_of_squares(const float (&x)[EPT]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < EPT; ++k) s = __fmaf_rn(x[k], x[k], s);
+  if ((s >= 0x1p-100f && s < INFINITY) || s != s) return static_cast<double>(s);
+  uint32_t any = 0;
+#pragma unroll
+  for (int k = 0; k < EPT; ++k) any |= __float_as_uint(x[k]) << 1;
+  double d = 0.0;
+  if (any != 0) {
+#pragma unroll
+    for (int k = 0; k < EPT; ++k) d = __fma_rn(static_cast<double>(x[k]), static_cast<double>(x[k]), d);
+  }
+  return d;
+}
+
 // squares are summed eight at a time in fp32 and from there on in fp64, in an order that does not
 // depend on the run
 template <int DT, int CAP>
@@ -353,11 +372,9 @@ __global__ void __launch_bounds__(THREADS) multi_norm_kernel(const __grid_consta
     }
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-      float x[EPT], s = 0.0f;
+      float x[EPT];
       raw[u].get(x);
-#pragma unroll
-      for (int k = 0; k < EPT; ++k) s = __fmaf_rn(x[k], x[k], s);
-      sum += static_cast<double>(s);
+      sum += sum_of_squares(x);
     }
   }
   const double t = block_sum_d(sum, red);
@@ -374,7 +391,8 @@ __global__ void __launch_bounds__(1024) multi_norm_final_kernel(const double* pa
     const float r = static_cast<float>(sqrt(s));
     *norm = r;
     if (coef != nullptr) {
-      const float q = max_norm / (r + 1e-6f);
+      // (a norm beyond fp32 still has a factor, if a subnormal one: with r = inf it would be 0 and every gradient lost)
+      const float q = isinf(r) && !isinf(s) ? static_cast<float>(max_norm / sqrt(s)) : max_norm / (r + 1e-6f);
       *coef = q > 1.0f ? 1.0f : q;              // a NaN stays one
     }
   }

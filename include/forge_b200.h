@@ -392,7 +392,8 @@ int forge_multi_adamw(const ForgeMultiArgs* args, void* cuda_stream);
 
 /* norm = sqrt of the sum of the squares of all elements of a list of gradients, and, if `coef` is given,
  * coef = min(1, max_norm / (norm + 1e-6)) (the factor of torch.nn.utils.clip_grad_norm_); both device
- * scalars.  Sums are fp64 from eight elements up, in a fixed order.  scratch: 8-byte aligned. */
+ * scalars.  Sums are fp64 from eight elements up (and for squares outside fp32's range), in a fixed order; a norm above
+ * fp32's range is inf, its coef is right.  scratch: 8-byte aligned. */
 typedef struct ForgeNormItem {
   const void* grad;
   int64_t numel;

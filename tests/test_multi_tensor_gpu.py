@@ -420,3 +420,30 @@ def test_refusals():
             MultiTensorAdamW([torch.nn.Parameter(p)], **kw)
     with pytest.raises(ValueError):
         MultiTensorAdamW([torch.nn.Parameter(p)]).pre_step()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [1e20, 3e38, 1e-20, 1e-30, 1e-38])
+def test_norm_of_gradients_whose_squares_leave_fp32(dtype, scale):
+    """Against 64 bits; the norm itself is rounded to fp32 (and is infinite where it exceeds its range).  Eight squares in fp32 are
+    off by 8 2^-24 of their sum at most, the root by half of that."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    big = torch.rand(70001, device=DEV, generator=g) * scale                 # up to `scale`, the type's normal range and a bit below
+    grads = [big.to(dtype), (torch.rand(13, device=DEV, generator=g) * min(scale, 1.0)).to(dtype), torch.zeros(4096, device=DEV, dtype=dtype)]
+    exact = math.sqrt(sum(float(t.double().square().sum()) for t in grads))
+    norm, coef = multi_tensor_grad_norm(grads, 0.5)
+    if exact > torch.finfo(torch.float32).max:
+        assert norm.isinf() and abs(float(coef) - 0.5 / exact) <= 2.0 ** -149        # (a subnormal number)
+    else:
+        assert abs(float(norm) - exact) <= 2.0 ** -21 * exact + 2.0 ** -149
+        assert abs(float(coef) - min(1.0, 0.5 / (exact + 1e-6))) <= 1e-6 * min(1.0, 0.5 / (exact + 1e-6)) + 2.0 ** -149
+    one = torch.zeros(9, device=DEV, dtype=dtype)
+    one[4] = scale
+    want = float(one.double().norm())
+    norm, coef = multi_tensor_grad_norm([one], 1.0)
+    assert abs(float(norm) - want) <= 2e-7 * want
+    # a step clipped by it moves the parameters
+    p, m, v = torch.zeros(9, device=DEV), torch.zeros(9, device=DEV), torch.zeros(9, device=DEV)
+    if scale > 1:
+        multi_tensor_adamw([p], [one], [m], [v], max_norm=1.0, weight_decay=0.0)
+        assert abs(float(m[4]) - 0.1) < 1e-6 and p[4] < 0
