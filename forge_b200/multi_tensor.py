@@ -210,14 +210,21 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 del self.state[p]
                 raise RuntimeError("the moments are created (zeroed) in the first step: run one step before it is captured")
             dt, dev = _DTYPE_OF[mode], p.device
-            st["step"] = 0
-            st["exp_avg"] = torch.zeros(p.shape, dtype=dt, device=dev)
-            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=dt, device=dev)
+            new = {k: torch.empty(p.shape, dtype=dt, device=dev) for k in ("exp_avg", "exp_avg_sq")}
             if dt in _QUANTIZED:
-                blocks = -(-p.numel() // QBLOCK)
-                st["exp_avg_scale"] = torch.ones(blocks, dtype=torch.float32, device=dev)
-                st["exp_avg_sq_scale"] = torch.ones(blocks, dtype=torch.float32, device=dev)
+                for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+                    new[k] = torch.empty(-(-p.numel() // QBLOCK), dtype=torch.float32, device=dev)
+            self._start(new)
+            st.update(new)
         return st
+
+    @staticmethod
+    def _start(st):
+        """What the first step begins with, written to the tensors of a parameter's state."""
+        st["step"] = 0
+        for k, t in st.items():
+            if k != "step":
+                t.fill_(1.0) if k.endswith("_scale") else t.zero_()
 
     def enable_device_hyper(self):
         if self._device_hyper is None:             # (captured steps read the blocks that are there)
@@ -308,21 +315,35 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As in ``torch.optim``, but the moments keep the types they were saved in (the base class would cast them to the
         parameters' type), and are loaded into the tensors that are there where those fit: a captured ``step()`` goes on
-        with them."""
+        with them.  Moments of a parameter that the checkpoint lacks stay as well and start again from zero.  After
+        ``enable_device_hyper()`` a checkpoint that does not fit the moments (another ``state_mode``) is refused."""
         there = dict(self.state)
+        pairs = [(p, state_dict["state"].get(index)) for group, saved in zip(self.param_groups, state_dict["param_groups"])
+                 for p, index in zip(group["params"], saved["params"])]
+        if self._device_hyper is not None:
+            for p, st in pairs:
+                old = there.get(p)
+                for k in {*old, *st} if old and st else ():
+                    if k != "step" and not self._fits(old.get(k), st.get(k), p.device):
+                        raise ValueError(f"{k} of the checkpoint does not fit the moments that a captured step may be using; load it "
+                                         f"before enable_device_hyper(), or into another optimizer")
         super().load_state_dict(state_dict)
-        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
-            for p, index in zip(group["params"], saved["params"]):
-                st = state_dict["state"].get(index)
-                if st:
-                    old = there.get(p, {})
-                    self.state[p] = {k: self._load(old.get(k), v, p.device) for k, v in st.items()}
+        for p, st in pairs:
+            old = there.get(p, {})
+            if st:
+                self.state[p] = {k: self._load(old.get(k), v, p.device) for k, v in st.items()}
+            elif old:
+                self._start(old)
+                self.state[p] = old
         self._device_step = max((st["step"] for st in self.state.values() if st), default=0)
 
     @staticmethod
-    def _load(old, new, device):
+    def _fits(old, new, device):
+        return (isinstance(old, torch.Tensor) and isinstance(new, torch.Tensor) and old.shape == new.shape and old.dtype == new.dtype
+                and old.device == device)
+
+    @classmethod
+    def _load(cls, old, new, device):
         if not isinstance(new, torch.Tensor):
             return copy.deepcopy(new)
-        if isinstance(old, torch.Tensor) and old.shape == new.shape and old.dtype == new.dtype and old.device == device:
-            return old.copy_(new)
-        return new.to(device, copy=True)
+        return old.copy_(new) if cls._fits(old, new, device) else new.to(device, copy=True)

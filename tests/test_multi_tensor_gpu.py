@@ -447,3 +447,30 @@ def test_norm_of_gradients_whose_squares_leave_fp32(dtype, scale):
     if scale > 1:
         multi_tensor_adamw([p], [one], [m], [v], max_norm=1.0, weight_decay=0.0)
         assert abs(float(m[4]) - 0.1) < 1e-6 and p[4] < 0
+
+
+def test_a_captured_step_goes_on_where_a_checkpoint_lacks_a_parameter():
+    a = _params(7, torch.bfloat16)
+    opt = MultiTensorAdamW(a, lr=1e-2, state_mode="int8")
+    _give_grads(a, 0)
+    opt.step()
+    opt.enable_device_hyper()
+    graph = torch.cuda.CUDAGraph()
+    opt.pre_step()
+    with torch.cuda.graph(graph):
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    del saved["state"][1]
+    saved["state"][0]["step"] = saved["state"][2]["step"] = 4
+    opt.load_state_dict(saved)
+    b = [p.detach().clone() for p in a]
+    states = [{k: v.clone() for k, v in opt.state[p].items() if k != "step"} for p in a]
+    assert (states[1]["exp_avg"] == 0).all() and (states[1]["exp_avg_sq_scale"] == 1).all()
+    opt.pre_step()
+    graph.replay()
+    for p, q, st in zip(a, b, states):
+        multi_tensor_adamw([q], [p.grad], [st["exp_avg"]], [st["exp_avg_sq"]], [st["exp_avg_scale"]], [st["exp_avg_sq_scale"]],
+                           lr=1e-2, step=5)
+        assert torch.equal(p, q)
+        for k, v in st.items():
+            assert torch.equal(opt.state[p][k], v)

@@ -221,3 +221,51 @@ def test_logprobs_row_maxima_and_sums_are_checked():
         assert lib.forge_logprobs_backward(ctypes.byref(logprobs(**kw)), P, P, P, 100, None) == code
     assert lib.forge_logprobs_forward(ctypes.byref(logprobs(row_max=P + 2)), None) == _lib.FORGE_ERR_ALIGNMENT
     assert lib.forge_logprobs_join(ctypes.byref(logprobs(log_sum=P + 2)), P, P, 2, None) == _lib.FORGE_ERR_ALIGNMENT
+
+
+@pytest.mark.parametrize("mode", ["f32", "bf16", "int8", "fp8_block"])
+def test_loading_a_checkpoint_keeps_the_moments_where_they_are(mode):
+    """A captured step goes on with the tensors that it was captured with: a checkpoint is loaded into them, and those of a
+    parameter that it lacks start again from what the first step begins with."""
+    import copy
+    from forge_b200.multi_tensor import MultiTensorAdamW
+    params = [torch.nn.Parameter(torch.ones(3, 70)), torch.nn.Parameter(torch.ones(5))]
+    opt = MultiTensorAdamW(params, state_mode=mode)
+    fresh = [{k: v.clone() if k != "step" else v for k, v in opt._state_of(p, mode).items()} for p in params]
+    for p in params:
+        for k, v in opt.state[p].items():
+            if k == "step":
+                opt.state[p][k] = 7
+            else:
+                v.view(torch.uint8).fill_(9)
+    before = {p: dict(opt.state[p]) for p in params}
+    saved = copy.deepcopy(opt.state_dict())
+    del saved["state"][1]
+    opt.load_state_dict(saved)
+    for p in params:
+        for k, v in before[p].items():
+            if k != "step":
+                assert opt.state[p][k] is v
+    assert opt.state[params[0]]["step"] == 7 and opt.state[params[1]]["step"] == 0
+    for k, v in fresh[1].items():
+        if k != "step":
+            assert torch.equal(opt.state[params[1]][k].view(torch.uint8), v.view(torch.uint8))
+            assert (opt.state[params[0]][k].view(torch.uint8) == 9).all()
+
+
+def test_a_checkpoint_that_does_not_fit_a_captured_step_is_refused():
+    import copy
+    from forge_b200.multi_tensor import MultiTensorAdamW
+    p = torch.nn.Parameter(torch.ones(3, 70))
+    old, new = MultiTensorAdamW([p], lr=0.5, state_mode="int8"), MultiTensorAdamW([p], lr=1.0, state_mode="f32")
+    old._state_of(p, "int8"), new._state_of(p, "f32")
+    saved = copy.deepcopy(old.state_dict())
+    new.enable_device_hyper()                          # what a captured step reads may be in use
+    state = new.state[p]["exp_avg"]
+    with pytest.raises(ValueError, match="exp_avg"):
+        new.load_state_dict(saved)
+    assert new.state[p]["exp_avg"] is state and new.param_groups[0]["lr"] == 1.0
+    again = MultiTensorAdamW([p], lr=1.0, state_mode="f32")
+    again._state_of(p, "f32")
+    again.load_state_dict(saved)                       # without one it is taken as it is
+    assert again.state[p]["exp_avg"].dtype == torch.int8 and again.param_groups[0]["state_mode"] == "int8"
