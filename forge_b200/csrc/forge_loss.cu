@@ -746,9 +746,10 @@ static int check(const ForgeLogprobsArgs& a, const char* what) {
   if (a.rows < 0 || a.vocab < 0) return fail(FORGE_ERR_INVALID_ARG, "%s: negative dimension", what);
   if (a.dtype != FORGE_DT_BF16 && a.dtype != FORGE_DT_F32) return fail(FORGE_ERR_INVALID_ARG, "%s: unknown dtype %d", what, a.dtype);
   if (a.top_k < 0 || a.top_k > MAX_TOP) return fail(FORGE_ERR_INVALID_ARG, "%s: top_k must be 0 .. %d (got %d)", what, MAX_TOP, a.top_k);
-  if (!(a.temperature > 0.0) || !isfinite(a.temperature) || !isfinite(1.0f / static_cast<float>(a.temperature)) ||
-      static_cast<float>(a.temperature) == 0.0f)
-    return fail(FORGE_ERR_INVALID_ARG, "%s: temperature must be a positive finite number (got %g)", what, a.temperature);
+  // log2 e / temperature is a number in fp32, and the exponential of the lowest logit over the temperature 0: a masked (-inf)
+  // logit is taken for one of those
+  if (!(a.temperature >= 1e-36 && a.temperature <= 1e36))
+    return fail(FORGE_ERR_INVALID_ARG, "%s: temperature must be a positive number, 1e-36 .. 1e36 (got %g)", what, a.temperature);
   if (a.vocab_start < 0 || a.vocab_total < a.vocab_start + a.vocab || a.vocab_total > 0x7fffffffll)
     return fail(FORGE_ERR_SHAPE, "%s: columns [%lld, %lld) of a vocabulary of %lld", what, (long long)a.vocab_start,
                 (long long)(a.vocab_start + a.vocab), (long long)a.vocab_total);

@@ -223,8 +223,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], *, top
     process group calls with its own slice of the same rows (collective: two small all-gathers), and the results are the
     same on every rank.  The gradient is that of this rank's columns for the gradients that reach this rank's results."""
     temperature = float(temperature)
-    if not temperature > 0 or temperature == float("inf"):
-        raise ValueError(f"temperature must be a positive finite number (got {temperature})")
+    if not 1e-36 <= temperature <= 1e36:
+        raise ValueError(f"temperature must be a positive number, 1e-36 .. 1e36 (got {temperature})")
     if group is None and (vocab_start != 0 or vocab_total is not None and vocab_total != logits.shape[-1]):
         raise ValueError("a slice of the vocabulary needs the process group of the other slices")
     if group is not None and vocab_total is None:

@@ -336,7 +336,7 @@ typedef struct ForgeLogprobsArgs {
   int64_t rows, vocab, ld;
   int64_t vocab_start, vocab_total;
   int64_t ignore_index;
-  double temperature;
+  double temperature;        /* 1e-36 .. 1e36                                                           */
   int32_t dtype;             /* FORGE_DT_* of logits (and of the gradient)                              */
   int32_t top_k;
   float* logprobs;           /* (rows,); outputs may be NULL except those of top_k                      */

@@ -190,3 +190,27 @@ def test_gradient_of_a_row_of_the_lowest_value(dtype, temperature):
     assert ((dx.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 12 * 2.0 ** -22 + 2.0 ** -22) * want.abs() + 2.0 ** -23 / temperature / vocab).all()
     (dx,) = torch.autograd.grad(out.entropy.sum(), x)
     assert (dx.double().abs() <= 2 * 2.0 ** -21 * log_v / vocab / temperature).all()
+
+
+@pytest.mark.parametrize("mask", ["inf", "lowest"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_extreme_temperatures(dtype, mask):
+    """At 1e36 every logit that is not masked is as likely as the next, at 1e-36 the largest has all of the probability."""
+    x, t = make(5, 3001, dtype, seed=55, masked=0.4)
+    hidden = x == -math.inf
+    if mask == "lowest":
+        x = lowest(x, dtype)
+    x[:, 7] = 20.0
+    hidden[:, 7] = False
+    t[0], t[1] = 7, 0
+    x = x.requires_grad_(True)
+    left = (~hidden).sum(1).double()
+    out = token_logprobs(x, t, temperature=1e36)
+    at = hidden.gather(1, t[:, None])[:, 0]
+    assert ((out.logprobs.double() + left.log()).abs() <= 2.0 ** -20 * left.log())[~at].all() and (out.logprobs[at] < -100).all()
+    assert ((out.entropy.double() - left.log()).abs() <= 2.0 ** -20 * left.log()).all()
+    cold = token_logprobs(x, t, temperature=1e-36, top_k=1)
+    close(cold.logprobs, (x.detach().double().gather(1, t[:, None])[:, 0] - 20.0) / 1e-36, torch.zeros(5, device=DEV))
+    assert (cold.entropy == 0).all() and (cold.top_ids == 7).all() and (cold.top_logprobs == 0).all()
+    (dx,) = torch.autograd.grad(cold.entropy.sum(), x)
+    assert (dx == 0).all()

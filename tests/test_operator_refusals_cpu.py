@@ -269,3 +269,15 @@ def test_a_checkpoint_that_does_not_fit_a_captured_step_is_refused():
     again._state_of(p, "f32")
     again.load_state_dict(saved)                       # without one it is taken as it is
     assert again.state[p]["exp_avg"].dtype == torch.int8 and again.param_groups[0]["state_mode"] == "int8"
+
+
+@pytest.mark.parametrize("temperature", [3.4e-39, 1e-37, 1e37, 1e300])
+def test_temperatures_that_leave_fp32_are_refused(temperature):
+    """log2 e / temperature has to be a number, and (lowest logit) / temperature far below the exponential's range."""
+    bad, a = _lib.FORGE_ERR_INVALID_ARG, logprobs(temperature=temperature)
+    assert _lib.load().forge_logprobs_forward(ctypes.byref(a), None) == bad
+    assert _lib.load().forge_logprobs_join(ctypes.byref(a), P, P, 2, None) == bad
+    assert _lib.load().forge_logprobs_backward(ctypes.byref(a), P, P, P, 100, None) == bad
+    from forge_b200.loss import token_logprobs
+    with pytest.raises(ValueError, match="temperature"):
+        token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.long), temperature=temperature)
