@@ -70,10 +70,18 @@ def rest_optimizer(args, params):
     return opt.enable_device_hyper() if args.graph else opt
 
 
-def pre_step(opt):
-    """Hyper-parameters of the coming step to the device, where the optimizer reads them from there."""
-    if getattr(opt, "reads_device_hyper", False):
-        opt.pre_step()
+def step_counter(opt):
+    """A function of the step's number to call before it: hyper-parameters to the device, where the optimizer reads them from
+    there.  That counts the step, so a step that comes by again (its capture has failed) is left alone."""
+    last = None
+
+    def pre_step(step):
+        nonlocal last
+        if getattr(opt, "reads_device_hyper", False) and step != last:
+            opt.pre_step()
+        last = step
+
+    return pre_step
 
 
 def main():
@@ -148,6 +156,7 @@ def main():
         if args.graph:
             manager.enable_device_hyper(dev)
         opt = rest_optimizer(args, manager.get_non_fused_params())
+    pre_step = step_counter(opt)
 
     torch.cuda.reset_peak_memory_stats(dev)
     times, losses = [], []
@@ -184,7 +193,7 @@ def main():
             static_ids.copy_(ids)
             if manager is not None:
                 manager.pre_step(lr=1e-4, weight_decay=0.01)
-            pre_step(opt)
+            pre_step(step)
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 static_loss.copy_(one_step(static_ids).detach())
@@ -196,7 +205,7 @@ def main():
         t0 = time.perf_counter()
         if manager is not None:
             manager.pre_step(lr=1e-4, weight_decay=0.01)
-        pre_step(opt)
+        pre_step(step)
         if graph is not None:
             static_ids.copy_(ids)
             graph.replay()
@@ -263,6 +272,7 @@ def run_tp(args):
     if args.graph:
         manager.enable_device_hyper(dev)
     opt = rest_optimizer(args, manager.get_non_fused_params())
+    pre_step = step_counter(opt)
     head_norms = model.head_sharded_norm_params()
     n_local = sum(p.numel() for p in model.parameters())
     n_sharded = sum(m.weight.numel() for m in manager._fused_modules)
@@ -296,7 +306,7 @@ def run_tp(args):
         if args.graph and graph is None and step == 2:
             static_ids.copy_(ids)
             manager.pre_step(lr=1e-4, weight_decay=0.01)
-            pre_step(opt)
+            pre_step(step)
             try:
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph):
@@ -317,7 +327,7 @@ def run_tp(args):
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
         manager.pre_step(lr=1e-4, weight_decay=0.01)
-        pre_step(opt)
+        pre_step(step)
         if graph is not None:
             static_ids.copy_(ids)
             graph.replay()
