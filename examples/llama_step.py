@@ -121,6 +121,10 @@ def main():
                     help="single GPU: forward products and input gradients of the fused linears in e4m3 with block scales")
     ap.add_argument("--no-group", action="store_true", help="one launch per linear instead of one per decoder layer")
     args = ap.parse_args()
+    if args.fp8_products and (args.tp or args.baseline):
+        ap.error("--fp8-products is for the fused linears of a single GPU (not with --tp or --baseline)")
+    if args.rest_state and args.baseline:
+        ap.error("--baseline leaves every parameter to torch.optim.AdamW (no --rest-state)")
     if args.tp:
         return run_tp(args)
 
