@@ -198,6 +198,7 @@ def main():
             if manager is not None:
                 manager.pre_step(lr=1e-4, weight_decay=0.01)
             pre_step(step)
+            loss = None                       # no eager graph of the same leaves is alive during the capture
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 static_loss.copy_(one_step(static_ids).detach())
@@ -311,6 +312,7 @@ def run_tp(args):
             static_ids.copy_(ids)
             manager.pre_step(lr=1e-4, weight_decay=0.01)
             pre_step(step)
+            loss = None                       # no eager graph of the same leaves is alive during the capture
             try:
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph):
