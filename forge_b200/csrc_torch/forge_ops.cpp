@@ -23,10 +23,15 @@ namespace py = pybind11;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// the exceptions of forge_b200._lib.check
 void check(int rc, const char* what) {
+  if (rc == FORGE_OK) return;
   if (rc == FORGE_ERR_INVALID_ARG || rc == FORGE_ERR_SHAPE || rc == FORGE_ERR_UNSUPPORTED)
     TORCH_CHECK_VALUE(false, what, ": ", forge_last_error_string(), " (code ", rc, ")");
-  TORCH_CHECK(rc == FORGE_OK, what, ": ", forge_last_error_string(), " (code ", rc, ")");
+  const std::string message = c10::str(what, ": ", forge_last_error_string(), " (code ", rc, ")");
+  py::gil_scoped_acquire gil;                // (a backward pass runs without it)
+  py::set_error(py::module_::import("forge_b200._lib").attr("ForgeLibraryError"), message.c_str());
+  throw py::error_already_set();
 }
 
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(); }

@@ -474,3 +474,28 @@ def test_a_captured_step_goes_on_where_a_checkpoint_lacks_a_parameter():
         assert torch.equal(p, q)
         for k, v in st.items():
             assert torch.equal(opt.state[p][k], v)
+
+
+@pytest.mark.parametrize("direct", [True, False])
+def test_errors_are_the_same_on_both_paths(direct, monkeypatch):
+    """A code of the library is the same exception from the extension and from Python."""
+    from forge_b200 import native
+    monkeypatch.setenv("FORGE_NATIVE_AUTOGRAD", "1" if direct else "0")
+    native.reset()
+
+    class Hyper:                                         # off its boundary: refused by the host code, never read
+        dev = torch.zeros(16, device=DEV)
+
+        def data_ptr(self):
+            return self.dev.data_ptr() + 4
+
+    try:
+        assert (native.module() is not None) == direct
+        p, g, m, v = (torch.zeros(8, device=DEV) for _ in range(4))
+        with pytest.raises(_lib.ForgeLibraryError, match="hyper_device is not aligned"):
+            multi_tensor_adamw([p], [g], [m], [v], hyper_device=Hyper())
+        with pytest.raises(ValueError, match="step must be"):
+            multi_tensor_adamw([p], [g], [m], [v], step=0)
+    finally:
+        monkeypatch.undo()
+        native.reset()
