@@ -50,6 +50,10 @@ at::Tensor once(const at::Tensor& g) {
   return (*node)({g})[0];
 }
 
+// Saved tensors come back from whatever hooks are set on them (torch.autograd.graph.saved_tensors_hooks): in another layout,
+// perhaps, or as something else altogether, which is refused here as it would be at the operator's own entry.
+void check_saved(bool ok, const char* what) { TORCH_CHECK(ok, what, ": what was saved for the backward pass came back as something else"); }
+
 // ----- token log probabilities ---------------------------------------------------------------------
 struct Rows {
   int64_t rows, vocab, ld;
@@ -129,7 +133,7 @@ class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &t = saved[1];
+    at::Tensor x = saved[0], t = saved[1];
     variable_list none(5);
     if (!g[0].defined() && !g[1].defined()) return none;
     at::Tensor gr[2];
@@ -139,12 +143,23 @@ class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
     {
       at::NoGradGuard no_grad;
       Rows r;
-      as_rows(x, r);
+      x = as_rows(x, r) ? x : x.contiguous();
+      check_saved(as_rows(x, r), "token_logprobs");
       const int dev = x.get_device();
+      auto per_row_of = [&](const at::Tensor& s, at::ScalarType type) {
+        return s.is_cuda() && s.get_device() == dev && s.scalar_type() == type && s.numel() == r.rows;
+      };
+      check_saved(!t.defined() || per_row_of(t, at::kLong), "token_logprobs");
+      if (t.defined()) t = t.contiguous();
       c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
       ForgeLogprobsArgs a = loss_args(x, r, t, 0, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt());
       float** const per_row[3] = {&a.entropy, &a.row_max, &a.log_sum};
-      for (int i = 0; i < 3; ++i) *per_row[i] = static_cast<float*>(const_cast<void*>(saved[2 + i].const_data_ptr()));
+      at::Tensor rows[3];
+      for (int i = 0; i < 3; ++i) {
+        check_saved(per_row_of(saved[2 + i], at::kFloat), "token_logprobs");
+        rows[i] = saved[2 + i].contiguous();
+        *per_row[i] = static_cast<float*>(const_cast<void*>(rows[i].const_data_ptr()));
+      }
       dx = empty(x.sizes(), x.scalar_type(), x);
       check(forge_logprobs_backward(&a, gr[0].defined() ? static_cast<const float*>(gr[0].const_data_ptr()) : nullptr,
                                     gr[1].defined() ? static_cast<const float*>(gr[1].const_data_ptr()) : nullptr, dx.data_ptr(), r.vocab,
@@ -337,6 +352,14 @@ bool scale_matrix(const at::Tensor& t, int dev, int64_t rows, int64_t cols) {
 }
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 
+// saved codes whose rows no longer start on 16-byte boundaries (save_on_cpu brings them back without their pitch) get them again
+at::Tensor saved_codes(const at::Tensor& t, int dev) {
+  if (code_matrix(t, dev)) return t;
+  check_saved(t.is_cuda() && t.get_device() == dev && t.scalar_type() == at::kFloat8_e4m3fn && t.dim() == 2, "fp8_linear");
+  at::Tensor q = empty({t.size(0), (t.size(1) + 15) / 16 * 16}, at::kFloat8_e4m3fn, t).narrow(1, 0, t.size(1));
+  return q.copy_(t);
+}
+
 // contiguous x (..., K), quantised by rows, times the codes (N, K) of a weight -> (..., N) bf16
 at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ws) {
   const int dev = x.get_device();
@@ -386,7 +409,10 @@ class Fp8LinearFn : public torch::autograd::Function<Fp8LinearFn> {
     at::Tensor dx;
     {
       at::NoGradGuard no_grad;
-      dx = linear(g[0].contiguous(), saved[0], saved[1]);
+      const at::Tensor dy = g[0].contiguous(), codes = saved_codes(saved[0], dy.get_device());
+      check_saved(codes.size(1) == dy.size(-1) && scale_matrix(saved[1], dy.get_device(), blocks(codes.size(0)), blocks(codes.size(1))),
+                  "fp8_linear");
+      dx = linear(dy, codes, saved[1]);
     }
     out[0] = once(dx);
     return out;

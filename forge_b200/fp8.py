@@ -176,7 +176,14 @@ class _Fp8Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         dy2d = dy.reshape(-1, dy.shape[-1])
-        dx = _product(dy2d, *ctx.saved_tensors).view(ctx.shape) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            codes, scales = ctx.saved_tensors
+            if codes.dim() != 2 or codes.dtype != _CODE:
+                raise RuntimeError("fp8_linear: what was saved for the backward pass came back as something else")
+            if _pitch(codes) % 16 or codes.data_ptr() % 16:     # (save_on_cpu brings them back without their pitch)
+                codes = _empty_codes(*codes.shape, codes.device).copy_(codes)
+            dx = _product(dy2d, codes, scales).view(ctx.shape)
         db = dy2d.sum(0).to(ctx.bias_dtype) if ctx.needs_input_grad[1] else None
         return dx, db, None
 

@@ -192,7 +192,13 @@ class _TokenLogprobs(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_ent, _g_top, _g_ids):
         x, t, *saved = ctx.saved_tensors
+        _require_cuda(x, t, *saved)
         x = _rows(x)
+        # (hooks on saved tensors may have brought them back in another layout, or as something else)
+        t, saved = _targets(t), [s.contiguous() for s in saved]
+        if any(s.shape.numel() != x.shape[0] or s.dtype != torch.float32 or s.device != x.device for s in saved) or (
+                t is not None and (t.numel() != x.shape[0] or t.device != x.device)):
+            raise RuntimeError("token_logprobs: what was saved for the backward pass came back as something else")
         none = (None,) * 7
         if g_lp is None and g_ent is None:
             return (None, *none)

@@ -62,3 +62,51 @@ def test_8_bit_products_cannot_be_traced(path):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, (x,), check_trace=False)
     fp8_linear(x, w)
+
+
+def _strided(t):
+    """The same values in memory of another order."""
+    return t.detach().t().contiguous().t() if t.dim() == 2 else t.detach()
+
+
+@pytest.mark.parametrize("hooks", [torch.autograd.graph.save_on_cpu, lambda: torch.autograd.graph.saved_tensors_hooks(_strided, lambda t: t),
+                                   lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), _strided)])
+def test_saved_tensors_that_come_back_otherwise(path, hooks):
+    """Layouts that hooks on saved tensors change: rows become columns, pitches are lost."""
+    x = torch.randn(12, 264, device=DEV)
+    t = torch.randint(0, 200, (12,), device=DEV)
+    w = Fp8Weight.from_weight((torch.randn(392, 264, device=DEV)).bfloat16())       # codes_t: 264 rows of 392, pitch 400
+    dy = torch.randn(12, 392, device=DEV).bfloat16()
+
+    def results():
+        out = []
+        for view in (lambda v: v, lambda v: v[:, 3:250], lambda v: v.view(3, 4, 264)):
+            xr = x.clone().requires_grad_(True)
+            v = view(xr)
+            tt = t.view(v.shape[:-1])
+            o = token_logprobs(v, tt, top_k=2)
+            out += torch.autograd.grad(o.logprobs.sum() + o.entropy.sum(), xr)
+        xr = x.bfloat16().requires_grad_(True)
+        return out + list(torch.autograd.grad(fp8_linear(xr, w), xr, dy))
+
+    want = results()
+    with hooks():
+        got = results()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("wrong", [lambda t: t.cpu(), lambda t: t.to(torch.float64) if t.is_floating_point() else t,
+                                   lambda t: t.reshape(-1)[:-1] if t.numel() > 1 else t])
+def test_saved_tensors_that_are_something_else_are_refused(path, wrong):
+    x = torch.randn(12, 256, device=DEV).requires_grad_(True)
+    t = torch.randint(0, 256, (12,), device=DEV)
+    w = Fp8Weight.from_weight(torch.randn(128, 256, device=DEV).bfloat16())
+    xb = x.detach().bfloat16().requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.detach(), wrong):
+        out = token_logprobs(x, t)
+        y = fp8_linear(xb, w)
+        with pytest.raises((RuntimeError, ValueError, IndexError)):
+            out.logprobs.sum().backward()
+        with pytest.raises((RuntimeError, ValueError, IndexError)):
+            y.sum().backward()
