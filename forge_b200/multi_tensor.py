@@ -187,8 +187,6 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if not lr >= 0 or not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
             raise ValueError(f"lr={lr}, betas={betas}, eps={eps}, weight_decay={weight_decay}: out of range")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_mode=state_mode))
-        for group in self.param_groups:
-            self._check_group(group)
         self.max_grad_norm = max_grad_norm
         self.last_grad_norm = None
         self._device_hyper: dict[tuple, DeviceHyper] | None = None
@@ -200,8 +198,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise ValueError(f"Unknown state_mode: {group['state_mode']}. Use one of {STATE_MODES}.")
 
     def add_param_group(self, group):
+        self._check_group({**self.defaults, **group})
         super().add_param_group(group)
-        self._check_group(self.param_groups[-1])
 
     def _state_of(self, p, mode):
         st = self.state[p]

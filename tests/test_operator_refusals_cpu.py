@@ -281,3 +281,13 @@ def test_temperatures_that_leave_fp32_are_refused(temperature):
     from forge_b200.loss import token_logprobs
     with pytest.raises(ValueError, match="temperature"):
         token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.long), temperature=temperature)
+
+
+def test_a_refused_parameter_group_is_not_added():
+    from forge_b200.multi_tensor import MultiTensorAdamW
+    opt = MultiTensorAdamW([torch.nn.Parameter(torch.ones(3))], state_mode="int8")
+    with pytest.raises(ValueError, match="state_mode"):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(4))], state_mode="fp4"))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(4))]))
+    assert [g["state_mode"] for g in opt.param_groups] == ["int8", "int8"]
