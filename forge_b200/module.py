@@ -43,6 +43,7 @@ class FusedLinear(nn.Module):
     feeds it straight to the optimizer; the (out_features, in_features) gradient is never allocated."""
 
     _native_dgrad = False    # the use_forge_dgrad switch as last told to the C++ autograd node
+    fp8_products = False     # see use_fp8_products (here, so that modules pickled without it still run)
 
     def __init__(self, in_features, out_features, bias=False, optimizer_type="adamw",
                  quantize_state=False, state_mode=None, _adopt: nn.Linear | None = None,
@@ -73,8 +74,6 @@ class FusedLinear(nn.Module):
         self._l2_manager = None
         # False: materialise grad_W with a library GEMM and run the optimizer-only kernel
         self.use_fused_backward = True
-        # see use_fp8_products
-        self.fp8_products = False
         # set by FusedOptimizerManager.group_updates: the launch this module's update is issued with
         self._update_group = None
         # handle of the C++ autograd node (forge_b200.native), created on first use
