@@ -264,6 +264,6 @@ def test_peer_helpers_work_without_a_process_group():
 def test_modules_from_before_the_8_bit_products_still_run():
     """A whole module that was pickled by an earlier version has no `fp8_products` of its own."""
     m = FusedLinear(64, 32, bias=False).train()
-    del m.__dict__["fp8_products"]
+    m.__dict__.pop("fp8_products", None)
     x = torch.randn(3, 64)
     assert torch.equal(m(x), torch.nn.functional.linear(x, m.weight)) and not m.fp8_products
