@@ -384,9 +384,9 @@ __device__ __noinline__ u64 rescan(const Columns& c, int top_k) {
   return list;
 }
 
-// CTAs per SM: four of 64 registers (511 rows of 151936 fp32 logits take 69 us with three, 52 with four: one wave instead
-// of two).  With the top k three: the two registers that spill otherwise cost more than the fourth CTA brings (300 rows of
-// 128256 bf16 logits, k = 5: 32.5 against 37.4 us; 511 of 151936 fp32, k = 20, the other way: 80 against 73).
+// CTAs per SM: four of 64 registers (511 rows of 151936 fp32 logits take 69 us with three, 49 with four: one wave instead
+// of two).  With the top k three: fewer registers cost more than the fourth CTA brings (300 rows of
+// 128256 bf16 logits, k = 5: 31.2 against 33.8 us; 511 of 151936 fp32, k = 20, the other way: 79 against 71).
 template <int DT, bool TOP>
 __global__ void __launch_bounds__(THREADS, TOP ? 3 : 4) logprobs_kernel(const Params p, const int cs) {
   using V = Vec<DT>;

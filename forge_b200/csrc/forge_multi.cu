@@ -6,11 +6,12 @@
 // sums.  A thread owns 8 consecutive elements, so eight lanes own a quantisation block of 64 and agree on
 // its absmax with three shuffles; the blocks run over a tensor's elements in memory order, which for a
 // (V, H) weight with H % 64 == 0 is the layout of the fused path.  Same per-element arithmetic as the fused
-// path (forge_update.cuh), but for the scales of the 8-bit moments (block_scale there: at most one ulp apart).
+// path (forge_update.cuh), but for the scales of the 8-bit moments (block_scale there: at most one ulp apart).  As there,
+// an 8-bit second moment counts as at least 1e-8.
 //
 // Bound by memory: 3 element sizes of the parameter (read, write, gradient) and 2 of each moment.  A thread has the next
-// pass's elements on their way while it updates this one's: 525 M bf16 parameters with e4m3 moments take 830 us (6.5 TB/s),
-// 984 without; fp32 throughout, with the norm before it, 132 M take 640 us: 92 for the norm, which only reads (5.7 TB/s),
+// pass's elements on their way while it updates this one's: 525 M bf16 parameters with e4m3 moments take 830 us (6.5 TB/s; 931
+// where seconds of it have brought the SMs to the power cap), 984 without; fp32 throughout, with the norm before it, 132 M take 640 us: 92 for the norm, which only reads (5.7 TB/s),
 // and 541 for the update (6.8 TB/s).
 #include <cuda_bf16.h>
 

@@ -260,7 +260,8 @@ __device__ __forceinline__ float fp8blk_scale(float absmax) {
   return f_add(div_by_const<448>(absmax), 1e-12f);
 }
 // The rule of the multi-tensor step and of the 8-bit products: absmax times the rounded reciprocal of the largest
-// code, one instruction instead of the corrected quotient above and at most one ulp from it.
+// code, at most one ulp from the corrected quotient above.  Those kernels wait for memory either way (268 M parameters with int8
+// moments: 427 us, with the quotient 424): this is what their scales are defined as, not a saving.
 template <int TOP>
 __device__ __forceinline__ float block_scale(float absmax) {
   constexpr float r = 1.0f / static_cast<float>(TOP);

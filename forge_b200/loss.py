@@ -222,8 +222,9 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], *, top
     batch for one: give all positions and ``ignore_index`` as the last one's target instead), ``targets`` (...) integers
     or None.  A target equal to ``ignore_index`` gives 0 and no gradient of its own; one outside the vocabulary gives NaN,
     in the gradient too.  Logits of -inf have probability zero; rows of nothing else, or with NaN or +inf, give NaN as
-    ``log_softmax`` does.  Sums are fp32; the gradient comes in the logits' type, and a row neither of whose results has
-    one (an ignored target without an entropy gradient) gets zeros, whatever it holds.
+    ``log_softmax`` does; logits of the type's lowest value have probability zero beside any other, and are uniform among
+    themselves.  ``temperature``: 1e-36 .. 1e36.  Sums are fp32; the gradient comes in the logits' type, and a row neither of
+    whose results has one (an ignored target without an entropy gradient) gets zeros, whatever it holds.
 
     ``group``: the logits are this rank's columns ``[vocab_start, vocab_start + V)`` of ``vocab_total``, every rank of the
     process group calls with its own slice of the same rows (collective: two small all-gathers), and the results are the

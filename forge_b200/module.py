@@ -127,9 +127,10 @@ class FusedLinear(nn.Module):
         """Form the training forward product and the input gradient in e4m3 with one scale per block of 128
         (``forge_b200.fp8``): activations and output gradients are quantised by rows, the weight by 128 x 128 blocks, anew in
         every training forward.  The weight gradient and the update stay the fused kernel's, from the bf16 activations.  Pays
-        from a few thousand tokens per step on (quantising the weight costs two passes over it); between forward and
-        backward the transposed codes are kept, one byte per weight.  Evaluation uses the weight as it is.  No reference
-        counterpart."""
+        from about 2000 tokens per step on (two decoder layers of 4096 x 14336 with their embedding and lm_head: 6.9 ms instead of
+        6.0 at 512 tokens, 15.8 instead of 16.6 at 2048, 68.6 instead of 73.3 at 8192; quantising the weight costs two passes over
+        it); between forward and backward the transposed codes are kept, one byte per weight.  The output has the activations'
+        type.  Evaluation uses the weight as it is.  No reference counterpart."""
         if on and self.weight.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"fp8 products need a bfloat16 or float32 weight (got {self.weight.dtype})")
         self.fp8_products = bool(on)

@@ -7,7 +7,8 @@
     rest.step(); rest.zero_grad()
 
 One launch per combination of types and 448 tensors (``forge_multi_adamw``), with the arithmetic and the moment layouts of
-the fused path: fp32, bf16, int8 or e4m3 moments, the last two with one fp32 scale for each 64 consecutive elements.
+the fused path: fp32, bf16, int8 or e4m3 moments, the last two with one fp32 scale for each 64 consecutive elements and,
+as there, with a second moment of at least 1e-8 (gradients whose rms is below 1e-4 take the step that one of 1e-4 would).
 ``max_grad_norm`` scales the gradients by their common norm without a host synchronisation (``forge_multi_norm``).  The
 reference leaves these parameters to ``torch.optim`` (``src/fused_grad_optimizer/module.py:218-222``).
 """
@@ -56,7 +57,8 @@ def _one_device(tensors):
 
 def multi_tensor_grad_norm(grads, max_norm: float | None = None):
     """``(norm, coef)`` of a list of CUDA gradients, fp32 scalars on their device: the 2-norm of all elements and, with
-    ``max_norm``, ``min(1, max_norm / (norm + 1e-6))`` (None without).  Bit-reproducible; no host synchronisation."""
+    ``max_norm``, ``min(1, max_norm / (norm + 1e-6))`` (None without).  A norm above fp32's range reads as inf, its ``coef`` is
+    right; an infinite gradient gives 0.  Bit-reproducible; no host synchronisation."""
     nat = native.module()
     if nat is not None and (max_norm is None or max_norm > 0):
         out = nat.multi_norm(grads, max_norm or 0.0)

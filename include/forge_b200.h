@@ -368,7 +368,8 @@ int forge_logprobs_backward(const ForgeLogprobsArgs* args, const float* g_logpro
  * size and alignment; the moments follow `state_mode` (F32, BF16, INT8, FP8_BLOCK), the scales of the 8-bit
  * modes belong to 64 consecutive elements each (ceil(numel / 64) of them; the last block may be short), which
  * for a (V, H) weight with H % 64 == 0 is the layout of ForgeState; scale = absmax * fp32(1 / 127 or 1 / 448) + 1e-12, at
- * most one ulp from forge_optimizer_update's correctly rounded quotient.  The reference leaves these parameters to
+ * most one ulp from forge_optimizer_update's correctly rounded quotient.  With 8-bit moments the second one enters the
+ * step as max(v, 1e-8), as it does there.  The reference leaves these parameters to
  * torch.optim (src/fused_grad_optimizer/module.py:218-222).  Tensors must not overlap. */
 typedef struct ForgeMultiItem {
   void* param;
