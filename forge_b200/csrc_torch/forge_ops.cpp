@@ -118,8 +118,10 @@ std::array<at::Tensor, 6> loss_forward(const at::Tensor& x, const at::Tensor& t,
 
 class TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
  public:
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& t, int64_t top_k, double temperature,
-                               int64_t ignore) {
+  // (no targets: none, since an undefined tensor is no argument that apply() takes)
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& targets, int64_t top_k,
+                               double temperature, int64_t ignore) {
+    const at::Tensor t = targets.value_or(at::Tensor());
     auto out = loss_forward(x, t, top_k, temperature, ignore, true);
     ctx->save_for_backward({x, t, out[1], out[4], out[5]});
     ctx->saved_data["temperature"] = temperature;
@@ -184,7 +186,7 @@ py::object token_logprobs(const at::Tensor& x, const c10::optional<at::Tensor>& 
   const py::object none = py::none();
   auto wrap = [](const at::Tensor& v) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(v)); };
   if (at::GradMode::is_enabled() && x.requires_grad()) {
-    const auto out = TokenLogprobsFn::apply(x, t, top_k, temperature, ignore);
+    const auto out = TokenLogprobsFn::apply(x, t.defined() ? std::optional<at::Tensor>(t) : std::nullopt, top_k, temperature, ignore);
     return py::make_tuple(wrap(out[0]), wrap(out[1]), top_k ? wrap(out[2]) : none, top_k ? wrap(out[3]) : none);
   }
   const auto out = loss_forward(x, t, top_k, temperature, ignore, false);

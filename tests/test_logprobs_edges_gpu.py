@@ -214,3 +214,18 @@ def test_extreme_temperatures(dtype, mask):
     assert (cold.entropy == 0).all() and (cold.top_ids == 7).all() and (cold.top_logprobs == 0).all()
     (dx,) = torch.autograd.grad(cold.entropy.sum(), x)
     assert (dx == 0).all()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_entropy_gradient_without_targets(wide):
+    """No targets: the same as targets that are all ignored, in the direct call and the Python one."""
+    x, _ = make(6, 5000, torch.float32, seed=56)
+    x = torch.cat([x, x], 1)[:, :5000] if wide else x
+    t = torch.full((2, 3), -100, device=DEV)
+    grads = []
+    for targets in (None, t):
+        xr = x.detach().requires_grad_(True)
+        out = token_logprobs(xr.view(2, 3, 5000), targets, temperature=0.8)
+        assert (out.logprobs == 0).all()
+        grads += torch.autograd.grad((out.logprobs + out.entropy).sum(), xr)
+    assert torch.equal(*grads) and (grads[0] != 0).any()
