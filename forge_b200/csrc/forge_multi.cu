@@ -11,8 +11,8 @@
 //
 // Bound by memory: 3 element sizes of the parameter (read, write, gradient) and 2 of each moment.  A thread has the next
 // pass's elements on their way while it updates this one's: 525 M bf16 parameters with e4m3 moments take 830 us (6.5 TB/s; 931
-// where seconds of it have brought the SMs to the power cap), 984 without; fp32 throughout, with the norm before it, 132 M take 640 us: 92 for the norm, which only reads (5.7 TB/s),
-// and 541 for the update (6.8 TB/s).
+// where seconds of it have brought the SMs to the power cap), 984 without; fp32 throughout, with the norm before it, 132 M take
+// 640 us: about 90 for the norm, which only reads, and 541 for the update (6.8 TB/s).
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -8,7 +8,8 @@
 
 One launch per combination of types and 448 tensors (``forge_multi_adamw``), with the arithmetic and the moment layouts of
 the fused path: fp32, bf16, int8 or e4m3 moments, the last two with one fp32 scale for each 64 consecutive elements and,
-as there, with a second moment of at least 1e-8 (gradients whose rms is below 1e-4 take the step that one of 1e-4 would).
+as there, with a second moment of at least 1e-8 (where the gradients' rms is below 1e-4 the first moment is divided by
+1e-4, and the steps are smaller than AdamW's).
 ``max_grad_norm`` scales the gradients by their common norm without a host synchronisation (``forge_multi_norm``).  The
 reference leaves these parameters to ``torch.optim`` (``src/fused_grad_optimizer/module.py:218-222``).
 """
