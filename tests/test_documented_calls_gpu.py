@@ -298,3 +298,42 @@ def test_8_bit_products_under_every_optimizer_and_accumulation(optimizer, mode):
             assert p.isfinite().all() and not torch.equal(p, q) and p.grad is None
         results.append([p.detach() for p in net.parameters()])
     same(*results)
+
+
+def test_a_tensor_beyond_32_bits_is_updated_to_its_end():
+    n = 2 ** 31 + 2 ** 20 + 64 * 5 + 3
+    p = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    g = torch.full((n,), 0.5, dtype=torch.bfloat16, device=DEV)
+    m, v = (torch.zeros(n, dtype=torch.int8, device=DEV) for _ in range(2))
+    ms, vs = (torch.ones(-(-n // 64), device=DEV) for _ in range(2))
+    cuts = [(0, 6400), (2 ** 31 - 640, 2 ** 31 + 640), (n - 64 * 4 - n % 64, n)]
+    for i, (a, b) in enumerate(cuts):
+        p[a:b], g[a:b] = rows(b - a, seed=i).bfloat16(), rows(b - a, seed=i + 7).bfloat16()
+    parts = [[t[a:b].clone() for t in (p, g, m, v)] + [s[a // 64:-(-b // 64)].clone() for s in (ms, vs)] for a, b in cuts]
+    norm, coef = multi_tensor_grad_norm([g], 1.0)
+    exact = math.sqrt(sum(float(g[i:i + 2 ** 28].double().square().sum()) for i in range(0, n, 2 ** 28)))
+    assert abs(float(norm) - exact) <= 2.0 ** -21 * exact
+    multi_tensor_adamw([p], [g], [m], [v], [ms], [vs], grad_coef=coef, lr=1e-2)
+    multi_tensor_adamw(*([q[i] for q in parts] for i in range(6)), grad_coef=coef, lr=1e-2)
+    for (a, b), q in zip(cuts, parts):
+        same([t[a:b] for t in (p, g, m, v)] + [s[a // 64:-(-b // 64)] for s in (ms, vs)], q)
+    inner = p[10 ** 9:10 ** 9 + 64]
+    assert (inner == inner[0]).all() and inner[0] != 0
+
+
+def test_8_bit_products_beyond_32_bits():
+    """More than 2^31 codes of activations."""
+    tokens, n, k = 2 ** 20 + 2 ** 17 + 77, 136, 2048
+    x = torch.zeros(tokens, k, dtype=torch.bfloat16, device=DEV)
+    some = torch.tensor([0, 5, 2 ** 20 - 1, 2 ** 20, tokens - 200, tokens - 1], device=DEV)
+    x[some] = rows(6, k, seed=8).bfloat16()
+    w8 = Fp8Weight.from_weight(rows(n, k, seed=9).bfloat16())
+    y = fp8_linear(x, w8)
+    want = fp8_linear(x[some], w8)
+    # sums of the same terms in another order: 2^-24 of their absolute values each, and one rounding to bf16 each
+    xq, xs = quantize_fp8(x[some])
+    value = lambda q, s, r: q.double() * s.double().repeat_interleave(r, 0)[:q.shape[0]].repeat_interleave(128, 1)      # noqa: E731
+    size = value(xq, xs, 1).abs() @ value(w8.codes, w8.scales, 128).abs().t()
+    assert ((y[some].double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs() + 2.0 ** -23 * (131 + 16) * size).all()
+    y[some] = 0
+    assert (y == 0).all()
