@@ -675,8 +675,8 @@ __global__ void __launch_bounds__(BACK_THREADS) logprobs_backward_kernel(const B
   auto one = [&](float x) {
     const float y = __fmaf_rn(x - m, c, nl);
     const float pr = exp2_approx(y);
-    // (below -127 the probability is 0, and its logarithm must stay finite whatever b is)
-    if constexpr (ENT) return pr * __fmaf_rn(b, max_nan(y, -127.0f), a);
+    // (below -127 the probability is 0: p log p is then 0, too, however large b is)
+    if constexpr (ENT) return __fmaf_rn(pr * b, max_nan(y, -127.0f), pr * a);
     else return pr * a;
   };
   const int mis = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / ES;

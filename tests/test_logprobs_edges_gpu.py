@@ -229,3 +229,17 @@ def test_entropy_gradient_without_targets(wide):
         assert (out.logprobs == 0).all()
         grads += torch.autograd.grad((out.logprobs + out.entropy).sum(), xr)
     assert torch.equal(*grads) and (grads[0] != 0).any()
+
+
+@pytest.mark.parametrize("temperature,factor", [(1e-36, 100.0), (1e-30, 1e8), (0.5, 1e37)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_entropy_gradients_of_improbable_columns(dtype, temperature, factor):
+    """p log p is 0 where p is, also where factor / temperature times the logarithm leaves fp32."""
+    x = torch.zeros(3, 2000, device=DEV, dtype=dtype)
+    x[:, 1::2] = -200.0
+    x[:, 0] = 200.0
+    x = x.requires_grad_(True)
+    out = token_logprobs(x, None, temperature=temperature)
+    assert (out.entropy == 0).all()
+    (dx,) = torch.autograd.grad(out.entropy, x, torch.full((3,), factor, device=DEV))
+    assert (dx == 0).all()
